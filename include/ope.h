@@ -688,6 +688,102 @@ int ope_allreduce_enable_peer(int32_t peer_device);
 int ope_allreduce_flat(const ope_allreduce_ctx* ctx_host, uint32_t epoch, float* flat, int64_t n, int32_t* status, void* stream);
 int ope_allreduce_flat_dev(const ope_allreduce_ctx* ctx_host, uint32_t* epoch_state_dev, float* flat, int64_t n, int32_t* status, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Memory-block operators: what an agent with a wider or longer memory than the GRU of rnn.py:5-43 is made of. Each takes float32, bfloat16 or
+ * float16 tensors (OPE_F32 / OPE_BF16 / OPE_F16), computes in float32 and rounds once where it stores. No entry allocates, synchronises or
+ * keeps anything between calls; workspaces are the caller's, and a call may be recorded into a HIP graph.
+ * ---------------------------------------------------------------------------------------------- */
+#define OPE_F32 0
+#define OPE_BF16 1
+#define OPE_F16 2
+#define OPE_E4M3 3 /* 8-bit float, 4 exponent bits, largest value 448 */
+
+/* RMS norm with the residual's addition:  s = x + residual,  y = s * weight / sqrt(mean(s^2) + eps)  over rows of `width` elements.
+ *   x, residual  [rows][width] of `dtype`, rows x_stride / residual_stride ELEMENTS apart; residual may be NULL (s = x)
+ *   weight       [width] of `dtype`
+ *   y            [rows][width] contiguous, of `dtype` -- or, with out_dtype = OPE_E4M3, 8-bit values of y / scale[row],
+ *                scale[row] = max(max|y|, 448 * 2^-126) / 448 (float32; NaN where the row holds one)
+ *   sum_out      [rows][width] contiguous, s rounded to `dtype`; NULL = not wanted. May be `x` or `residual` itself where that is contiguous.
+ *   rstd         float32 [rows], 1 / sqrt(mean(s^2) + eps) for the backward pass; NULL = not wanted
+ * The norm is taken of the unrounded float32 sum. rows >= 0, 1 <= width <= 2^20. */
+typedef struct ope_norm_cfg {
+  int64_t rows, x_stride, residual_stride;
+  int32_t width, dtype, out_dtype;
+  float eps;
+} ope_norm_cfg;
+int ope_rms_norm(const ope_norm_cfg* cfg, const void* x, const void* residual, const void* weight, void* y, float* scale, void* sum_out,
+                 float* rstd, void* stream);
+/* Gradients:  h = weight * dy;  dx = rstd * (h - s * rstd^2 * mean(h * s)) + dsum  (the residual's gradient is the same tensor),
+ * dweight = sum over rows of dy * s * rstd, in a fixed order (no atomics).
+ *   dy, s, dx [rows][width] contiguous of cfg->dtype (s: sum_out of the forward call, or x itself, row stride x_stride); dsum likewise or NULL;
+ *   dweight [width] of cfg->dtype. dx may be dy or dsum. */
+int64_t ope_rms_norm_backward_workspace_bytes(const ope_norm_cfg* cfg);
+int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd,
+                          void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+/* Rows of x in 8 bits with one scale each (the scale rule above), e.g. the weights of ope_linear with 8-bit operands. cfg->eps, out_dtype and
+ * residual_stride are not read. */
+int ope_quantize_rows(const ope_norm_cfg* cfg, const void* x, void* q, float* scale, void* stream);
+
+/* Gated delta rule. Per sequence b and head h a state S [key_dim][value_dim] (float32), and per token t
+ *   S~ = exp(g_t) S;  u = beta_t (v_t - S~^T k_t);  S = S~ + k_t u^T;  o_t = scale * S^T q_t
+ *   q, k  [batch][seq_len][n_qk_heads][key_dim], v, o [batch][seq_len][n_heads][value_dim] of `dtype`, the last axis contiguous, the first
+ *         three with the strides given (in elements; a time-major batch is the same call with two strides exchanged). n_heads is a multiple
+ *         of n_qk_heads: query / key head i serves the value heads [i * r, (i + 1) * r), r = n_heads / n_qk_heads.
+ *   g     float32, log of the decay, beta float32: [batch][seq_len][n_heads], strides g_stride / beta_stride.
+ *         g = -inf clears the state in front of the token (an episode boundary inside a row).
+ *   lengths  int32 [batch] or NULL: tokens t >= lengths[b] (clamped to [0, seq_len]) are neither read nor do anything; their o is 0.
+ *   state0   float32 [batch][n_heads][key_dim][value_dim] or NULL (zeros); state_out the same shape: the state behind the last live token.
+ * The forward pass works on chunks of 64 tokens: with G the running sum of g inside a chunk, A_ij = beta_i exp(G_i - G_j) k_i.k_j (i > j),
+ *   (I + A) [W | U0] = [beta e^G k | beta v],  U = U0 - W S,  o = scale (e^G q S + tril(q k^T e^(G_i - G_j)) U),  S' = e^G_63 S + k^T e^(G_63 - G) U
+ * and leaves W, U and the chunks' first states in `saved` (ope_delta_saved_bytes), which the backward pass reads.
+ * key_dim 1..128, value_dim 1..1024. */
+typedef struct ope_delta_cfg {
+  int32_t batch, seq_len, n_heads, n_qk_heads, key_dim, value_dim, dtype;
+  float scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], g_stride[3], beta_stride[3]; /* batch, token, head */
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3], dg_stride[3], dbeta_stride[3];          /* read by ope_delta_backward only */
+} ope_delta_cfg;
+int64_t ope_delta_saved_bytes(const ope_delta_cfg* cfg);
+int64_t ope_delta_workspace_bytes(const ope_delta_cfg* cfg, int32_t backward);
+int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta,
+                      const float* state0, const int32_t* lengths, void* o, float* state_out, void* saved, int64_t saved_bytes,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients from d_o (of `dtype`, shape of o, strides o_stride) and d_state (float32, gradient of state_out; NULL = zeros): dq, dk (shape of q),
+ * dv (shape of v) of `dtype`, dg, dbeta float32, with the strides dq_stride .. dbeta_stride (last axis contiguous), d_state0 float32 or NULL.
+ * `saved` and the inputs are those of the forward call. Gradients of shared query / key heads are summed over their value heads in a fixed
+ * order. dg is 0 where g = -inf; everything is 0 behind a row's length. */
+int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta,
+                       const int32_t* lengths, const void* saved, int64_t saved_bytes, const void* d_o, const float* d_state, void* dq,
+                       void* dk, void* dv, float* dg, float* dbeta, float* d_state0, void* workspace, int64_t workspace_bytes, void* stream);
+/* One token: cfg->seq_len is not read, the token strides neither; `state` [batch][n_heads][key_dim][value_dim] is updated in place. */
+int ope_delta_step(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
+                   void* o, void* stream);
+
+/* Linear layer with its epilogue:  z = x w^T + bias,  y = act(z) + residual.
+ *   x [rows][in_width] rows x_stride elements apart, w [out_width][in_width] contiguous (torch.nn.Linear), both of `dtype`; y [rows][out_width]
+ *   contiguous, bias [out_width] and residual (rows residual_stride apart; bias / residual NULL = none) of out_dtype = dtype.
+ *   dtype = OPE_E4M3: 8-bit x and w with x_scale [rows] and w_scale [out_width] float32, z = x_scale w_scale x w^T + bias; out_dtype is one of
+ *   the other three. Forward only.
+ *   z_out [rows][out_width] contiguous or NULL: z rounded to out_dtype, what the backward pass needs where activation is not OPE_ACT_NONE.
+ * Products are summed in float32. Backward: dz = dy act'(z), dx = dz w, dw = dz^T x, dbias = sum over rows of dz (the residual's gradient is dy);
+ * dz is rounded to `dtype` for the products. dy, z contiguous; dx contiguous; dx, dw, dbias may be NULL (not wanted). Sums over rows are split in a
+ * way that follows from the sizes alone and added in a fixed order. in_width, out_width 1..2^20, rows >= 0. */
+#define OPE_ACT_NONE 0
+#define OPE_ACT_RELU 1
+#define OPE_ACT_TANH 2
+#define OPE_ACT_SILU 3
+#define OPE_ACT_GELU 4 /* z Phi(z) */
+typedef struct ope_linear_cfg {
+  int64_t rows, x_stride, residual_stride;
+  int32_t in_width, out_width, dtype, out_dtype, activation;
+} ope_linear_cfg;
+int64_t ope_linear_workspace_bytes(const ope_linear_cfg* cfg);
+int ope_linear(const ope_linear_cfg* cfg, const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
+               const void* residual, void* y, void* z_out, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t ope_linear_backward_workspace_bytes(const ope_linear_cfg* cfg);
+int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, const void* z, const void* x, const void* w, void* dx, void* dw, void* dbias,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -102,6 +102,24 @@ class MlpBatch(C.Structure):
                                           "valid_transition", "avail_acts", "next_avail_acts")]
 
 
+OPE_F32, OPE_BF16, OPE_F16, OPE_E4M3 = 0, 1, 2, 3
+
+
+class NormCfg(C.Structure):
+    _fields_ = [(k, C.c_int64) for k in ("rows", "x_stride", "residual_stride")] + [(k, C.c_int32) for k in ("width", "dtype", "out_dtype")] + [("eps", C.c_float)]
+
+
+class DeltaCfg(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("batch", "seq_len", "n_heads", "n_qk_heads", "key_dim", "value_dim", "dtype")] + [("scale", C.c_float)] + \
+               [(k + "_stride", C.c_int64 * 3) for k in ("q", "k", "v", "o", "g", "beta", "dq", "dk", "dv", "dg", "dbeta")]
+
+
+class LinearCfg(C.Structure):
+    _fields_ = [(k, C.c_int64) for k in ("rows", "x_stride", "residual_stride")] + \
+               [(k, C.c_int32) for k in ("in_width", "out_width", "dtype", "out_dtype", "activation")]
+
+
+OPERATOR_MIRRORS = {"ope_norm_cfg": NormCfg, "ope_delta_cfg": DeltaCfg, "ope_linear_cfg": LinearCfg}      # offpolicy_amd.ops
 ABI_MIRRORS = {"ope_live_target": LiveTarget, "ope_dims": Dims, "ope_fields": Fields, "ope_qmix_cfg": QmixCfg, "ope_gather_tune": GatherTune, "ope_obs_ref": ObsRef,
                "ope_adam_cfg": AdamCfg, "ope_ddpg_opt": DdpgOpt, "ope_ddpg_cfg": DdpgCfg, "ope_rddpg_cfg": RddpgCfg,
                "ope_allreduce_ctx": AllreduceCtx, "ope_mlp_batch": MlpBatch}
@@ -188,13 +206,27 @@ def _load():
         "ope_allreduce_enable_peer": (C.c_int, [i32]),
         "ope_allreduce_flat": (C.c_int, [C.POINTER(AllreduceCtx), C.c_uint32, p, i64, p, p]),
         "ope_allreduce_flat_dev": (C.c_int, [C.POINTER(AllreduceCtx), p, p, i64, p, p]),
+        # the operators' configurations travel as packed bytes (offpolicy_amd/ops/_common.py): a quarter of the cost of filling a ctypes struct
+        "ope_rms_norm": (C.c_int, [p] * 9),
+        "ope_rms_norm_backward_workspace_bytes": (i64, [p]),
+        "ope_rms_norm_backward": (C.c_int, [p] * 9 + [i64, p]),
+        "ope_quantize_rows": (C.c_int, [p] * 5),
+        "ope_delta_saved_bytes": (i64, [p]),
+        "ope_delta_workspace_bytes": (i64, [p, i32]),
+        "ope_delta_forward": (C.c_int, [p] * 11 + [i64, p, i64, p]),
+        "ope_delta_backward": (C.c_int, [p] * 8 + [i64] + [p] * 9 + [i64, p]),
+        "ope_delta_step": (C.c_int, [p] * 9),
+        "ope_linear_workspace_bytes": (i64, [p]),
+        "ope_linear": (C.c_int, [p] * 10 + [i64, p]),
+        "ope_linear_backward_workspace_bytes": (i64, [p]),
+        "ope_linear_backward": (C.c_int, [p] * 9 + [i64, p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)  # AttributeError here = a symbol declared in include/ope.h is missing
         fn.restype = res
         fn.argtypes = args
     # the mirror declarations above against the structs the library was compiled with: a drifted field would be read as garbage silently
-    for cname, cls in ABI_MIRRORS.items():
+    for cname, cls in list(ABI_MIRRORS.items()) + list(OPERATOR_MIRRORS.items()):
         want = lib.ope_abi_sizeof(cname.encode())
         if want != C.sizeof(cls):
             raise OpeError("%s: sizeof is %d in libope.so but %d in offpolicy_amd._lib.%s -- rebuild the library or fix the mirror"

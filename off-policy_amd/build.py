@@ -12,6 +12,11 @@ LIB = os.path.join(HERE, "libope.so")
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-Wall", "-Wno-unused-function",
          "-ffp-contract=off"]
+# The memory-block operators' sources: no v_pk_{add,mul,fma}_f32. -O3 forms them from ordinary float code, and some of their forms have
+# given wrong results on gfx950 now and then (the host pass warns that it does not know the feature: harmless). The training step's own
+# sources are built as they always were: its scan writes the packed form in asm, and without it the step takes 0.361 instead of 0.274 ms.
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+NO_PACKED_SOURCES = ("ope_delta", "ope_norm", "ope_linear")
 
 
 def sources():
@@ -60,7 +65,7 @@ def build(force=False, verbose=True, extra_flags=(), sanitize=False, experiments
         obj = os.path.join(odir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
         if force or _stale(obj, [src] + headers):
-            cmd = [hipcc] + flags + list(extra_flags) + ["-c", src, "-o", obj]
+            cmd = [hipcc] + flags + (NO_PACKED if os.path.basename(src).startswith(NO_PACKED_SOURCES) else []) + list(extra_flags) + ["-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd)))

@@ -1,0 +1,410 @@
+// Gated delta rule, forward: chunked over time for training and long inputs, one token at a time for acting (ope.h).
+//
+//   delta_prep   parallel over chunks: decays, A, the triangular solve for W and U0
+//   delta_scan   serial over chunks, parallel over (sequence, head, 16 value columns): U = U0 - W S, S' = e^G S + k^T e^.. U
+//   delta_out    parallel over chunks: o = scale (e^G q S + tril(q k^T decay) U)
+//   delta_step   one token: state read and written once
+#include "ope_delta.h"
+
+namespace ope {
+
+bool delta_ok(const ope_delta_cfg* c) {
+  if (!c || c->batch < 0 || c->seq_len < 0 || c->n_heads < 1 || c->n_qk_heads < 1 || c->n_heads % c->n_qk_heads) return false;
+  if (c->key_dim < 1 || c->key_dim > 128 || c->value_dim < 1 || c->value_dim > 1024 || !elem_float(c->dtype)) return false;
+  const DeltaDims d = delta_dims(c);
+  return (int64_t)d.B * d.H * (d.n > d.VT ? d.n : d.VT) < ((int64_t)1 << 31);     // workgroups of one launch
+}
+
+// Rows of one chunk-head: W = (I + A)^-1 beta e^G k, U0 = (I + A)^-1 beta v by block forward substitution, 16 columns a wave at a time.
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void delta_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ k_in, const T* __restrict__ v_in,
+                                                  const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
+                                                  float* __restrict__ W, float* __restrict__ WT, float* __restrict__ KdT, float* __restrict__ UT,
+                                                  float* __restrict__ gC) {
+  constexpr int Kp = 16 * KT;
+  __shared__ float k[kC][Kp + 4], NA[kC][kC + 4], inv[4][16][20];
+  __shared__ Gates gt;
+  const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
+  if (a.nv == 0) return;
+  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
+  load_rows<T, KT>(k, k_in, cfg.k_stride, a, a.h / (d.H / d.Hk), d.K);
+  __syncthreads();
+  minus_A<KT>(NA, k, gt);
+  if (threadIdx.x == 0) gC[a.c] = gt.whole;
+  __syncthreads();
+  if (w == 0) diag_inverse(inv, NA);
+  for (int q = threadIdx.x; q < Kp * 16; q += 256) {     // KdT: four tokens of one feature a thread
+    const int f = q / 16, t = (q % 16) * 4;
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = k[t + r][f] * gt.tail[t + r];
+    put4(&KdT[(a.c * Kp + f) * kC + t], v);
+  }
+  __syncthreads();
+  const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)a.t0 * cfg.v_stride[1] + a.h * cfg.v_stride[2];
+  for (int cg = w; cg < KT + d.VT; cg += 4) {
+    f32x4 x[4];
+    const int col = cg < KT ? 16 * cg + j : 16 * (cg - KT) + j;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * it + 4 * g + r;
+        float v = 0.f;
+        if (cg < KT) v = gt.head[t] * k[t][col];
+        else if (t < a.nv && col < d.V) v = (float)v0[(int64_t)t * cfg.v_stride[1] + col];
+        x[it][r] = gt.beta[t] * v;
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      f32x4 acc = x[it];
+#pragma unroll
+      for (int kt = 0; kt < it; ++kt) acc = mfma4(at4(&NA[16 * it + j][16 * kt + 4 * g]), x[kt], acc);
+      x[it] = mfma4(at4(&inv[it][j][4 * g]), acc, f32x4{0.f, 0.f, 0.f, 0.f});
+      if (cg < KT) {
+        put4(&WT[(a.c * Kp + col) * kC + 16 * it + 4 * g], x[it]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) W[(a.c * kC + 16 * it + 4 * g + r) * Kp + col] = x[it][r];
+      } else {
+        put4(&UT[(a.c * d.Vp + col) * kC + 16 * it + 4 * g], x[it]);
+      }
+    }
+  }
+}
+
+// The scan, forward or backward in time. Four waves share 16 value columns of one (sequence, head): wave w makes the 16 tokens 16w.. of
+// P = M1 S (64 x Kp times Kp x 16), then its share of the state's tiles of 16 keys. S lives in registers; it and U cross between the waves
+// through LDS, two barriers a chunk. The chain of a chunk is what bounds it, so the operands of the next one are loaded a chunk ahead.
+//   forward : U = U0 - W S;     S' = gC S + KdT U            M1 = W,  M2 = KdT
+//   backward: dU = dU0 + Kd dS'; dS = gC dS' + N - WT dU      M1 = Kd, M2 = WT
+template <int KT, bool BWD>
+__global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __restrict__ lengths, const float* __restrict__ M1,
+                                                  const float* __restrict__ M2, float* __restrict__ UT, float* __restrict__ ST,
+                                                  const float* __restrict__ gC, const float* __restrict__ first, float* __restrict__ last) {
+  constexpr int Kp = 16 * KT, NK = (KT + 3) / 4;      // tiles of keys a wave
+  __shared__ float SL[16][Kp + 4], UL[16][kC + 4];
+  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  const int vt = blockIdx.x % d.VT;
+  const int64_t bh = blockIdx.x / d.VT;
+  const int b = (int)(bh / d.H), v = 16 * vt + j;
+  const int n = ope_cdiv_dev(live_len(lengths, b, d.T), kC);
+  f32x4 S[NK];
+#pragma unroll
+  for (int q = 0; q < NK; ++q)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 16 * (w + 4 * q) + 4 * g + r;
+      S[q][r] = first && k < d.K && v < d.V ? first[(bh * d.K + k) * d.V + v] : 0.f;
+    }
+  f32x4 m1[KT], m2[NK][4], u, add[NK];
+  float whole = 0.f;
+  auto fetch = [&](int i) {
+    const int64_t c = bh * d.n + i;
+#pragma unroll
+    for (int q = 0; q < KT; ++q) m1[q] = at4(&M1[(c * kC + 16 * w + j) * Kp + 16 * q + 4 * g]);
+    u = at4(&UT[(c * d.Vp + v) * kC + 16 * w + 4 * g]);
+#pragma unroll
+    for (int q = 0; q < NK; ++q)
+      if (w + 4 * q < KT) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) m2[q][p] = at4(&M2[(c * Kp + 16 * (w + 4 * q) + j) * kC + 16 * p + 4 * g]);
+        if (BWD) add[q] = at4(&ST[(c * d.Vp + v) * Kp + 16 * (w + 4 * q) + 4 * g]);
+      }
+    whole = gC[c];
+  };
+  if (n > 0) fetch(BWD ? n - 1 : 0);
+  for (int s = 0; s < n; ++s) {
+    const int i = BWD ? n - 1 - s : s;
+    const int64_t c = bh * d.n + i;
+#pragma unroll
+    for (int q = 0; q < NK; ++q)
+      if (w + 4 * q < KT) {
+        const int k = 16 * (w + 4 * q) + 4 * g;
+        put4(&SL[j][k], S[q]);
+        put4(&ST[(c * d.Vp + v) * Kp + k], S[q]);
+      }
+    lds_barrier();
+    f32x4 p0 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < KT; ++q) p0 = mfma4(m1[q], at4(&SL[j][16 * q + 4 * g]), p0);
+    u = BWD ? u + p0 : u - p0;
+    put4(&UL[j][16 * w + 4 * g], u);
+    put4(&UT[(c * d.Vp + v) * kC + 16 * w + 4 * g], u);
+    lds_barrier();
+#pragma unroll
+    for (int q = 0; q < NK; ++q)
+      if (w + 4 * q < KT) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) acc = mfma4(m2[q][p], at4(&UL[j][16 * p + 4 * g]), acc);
+        S[q] = BWD ? whole * S[q] + add[q] - acc : whole * S[q] + acc;
+      }
+    if (s + 1 < n) fetch(BWD ? n - 2 - s : s + 1);
+  }
+#pragma unroll
+  for (int q = 0; q < NK; ++q)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 16 * (w + 4 * q) + 4 * g + r;
+      if (last && k < d.K && v < d.V) last[(bh * d.K + k) * d.V + v] = S[q][r];
+    }
+}
+
+// o of one chunk-head. Wave w owns the tokens 16w..: its rows of scale tril(q k^T decay) and of scale e^G q stay in registers while it walks
+// the value columns.
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void delta_out(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
+                                                 const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
+                                                 const float* __restrict__ ST, const float* __restrict__ UT, T* __restrict__ o) {
+  constexpr int Kp = 16 * KT;
+  __shared__ float q[kC][Kp + 4], k[kC][Kp + 4];
+  __shared__ Gates gt;
+  const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
+  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  T* o0 = o + a.b * cfg.o_stride[0] + (int64_t)a.t0 * cfg.o_stride[1] + a.h * cfg.o_stride[2];
+  const int rows = min(d.T - a.t0, kC);
+  if (a.nv == 0) {
+    for (int e = threadIdx.x; e < rows * d.V; e += 256) o0[(int64_t)(e / d.V) * cfg.o_stride[1] + e % d.V] = (T)0.f;
+    return;
+  }
+  if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
+  const int hk = a.h / (d.H / d.Hk);
+  load_rows<T, KT>(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows<T, KT>(k, k_in, cfg.k_stride, a, hk, d.K);
+  __syncthreads();
+  const int t = 16 * w + j;
+  f32x4 qs[KT], P[4];
+#pragma unroll
+  for (int c = 0; c < KT; ++c) qs[c] = at4(&q[t][16 * c + 4 * g]);
+#pragma unroll
+  for (int is = 0; is < 4; ++is) {
+    P[is] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (is <= w) {
+#pragma unroll
+      for (int c = 0; c < KT; ++c) P[is] = mfma4(at4(&k[16 * is + j][16 * c + 4 * g]), qs[c], P[is]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int s = 16 * is + 4 * g + r;
+        P[is][r] = s <= t ? cfg.scale * decay(gt, t, s) * P[is][r] : 0.f;
+      }
+    }
+  }
+  const float f = cfg.scale * gt.head[t];
+#pragma unroll
+  for (int c = 0; c < KT; ++c) qs[c] *= f;
+  for (int vt = 0; vt < d.VT; ++vt) {
+    const int v = 16 * vt + j;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KT; ++c) acc = mfma4(qs[c], at4(&ST[(a.c * d.Vp + v) * Kp + 16 * c + 4 * g]), acc);
+#pragma unroll
+    for (int is = 0; is < 4; ++is)
+      if (is <= w) acc = mfma4(P[is], at4(&UT[(a.c * d.Vp + v) * kC + 16 * is + 4 * g]), acc);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int tt = 16 * w + 4 * g + r;
+      if (tt < rows && v < d.V) o0[(int64_t)tt * cfg.o_stride[1] + v] = (T)(tt < a.nv ? acc[r] : 0.f);
+    }
+  }
+}
+
+// One token. A workgroup has 64 value columns of one (row, head): lane l of a wave 4 columns (l & 15), the keys dealt out over 16 groups of
+// 16 lanes. S passes through registers once: S^T k and S^T q in the same walk (o = e^g q.S + (q.k) u), then the update. Bound by memory.
+template <typename T, int NK>
+__global__ __launch_bounds__(256) void delta_step(ope_delta_cfg cfg, const T* __restrict__ q_in, const T* __restrict__ k_in, const T* __restrict__ v_in,
+                                                  const float* __restrict__ g_in, const float* __restrict__ beta_in, float* __restrict__ state,
+                                                  T* __restrict__ o) {
+  __shared__ float red[2][16][64];
+  __shared__ float qk_sh;
+  const int K = cfg.key_dim, V = cfg.value_dim, H = cfg.n_heads;
+  const int vb = ope_cdiv_dev(V, 64);
+  const int64_t bh = blockIdx.x / vb;
+  const int b = (int)(bh / H), h = (int)(bh % H), hk = h / (H / cfg.n_qk_heads);
+  const int grp = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4, v0 = (int)(blockIdx.x % vb) * 64 + c;
+  const T* qp = q_in + b * cfg.q_stride[0] + hk * cfg.q_stride[2];
+  const T* kp = k_in + b * cfg.k_stride[0] + hk * cfg.k_stride[2];
+  const float a = expf(g_in[b * cfg.g_stride[0] + h * cfg.g_stride[2]]);
+  const float beta = beta_in[b * cfg.beta_stride[0] + h * cfg.beta_stride[2]];
+  float* S0 = state + bh * K * V;
+  f32x4 S[NK], sk = {0.f, 0.f, 0.f, 0.f}, sq = sk;
+  float kk[NK], qk = 0.f;
+  const bool whole = v0 + 4 <= V;
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int k = grp + 16 * n;
+    S[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    kk[n] = 0.f;
+    if (k < K) {
+      const float* p = S0 + (int64_t)k * V + v0;
+      if (whole) S[n] = load_pack<float, 4>(p);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v0 + e < V) S[n][e] = p[e];
+      if (a == 0.f) S[n] = f32x4{0.f, 0.f, 0.f, 0.f};      // a reset forgets whatever the state holds
+      else S[n] *= a;
+      kk[n] = (float)kp[k];
+      const float qq = (float)qp[k];
+      qk = fmaf(qq, kk[n], qk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sk[e] = fmaf(S[n][e], kk[n], sk[e]);
+        sq[e] = fmaf(S[n][e], qq, sq[e]);
+      }
+    }
+  }
+  put4(&red[0][grp][c], sk);
+  put4(&red[1][grp][c], sq);
+  __shared__ float qks[16];
+  if ((threadIdx.x & 15) == 0) qks[grp] = qk;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float v = 0.f;
+    for (int i = 0; i < 16; ++i) v += qks[i];
+    qk_sh = v;
+  }
+  f32x4 u = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 16; ++i) u += at4(&red[0][i][c]);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (v0 + e < V) u[e] = beta * ((float)v_in[b * cfg.v_stride[0] + h * cfg.v_stride[2] + v0 + e] - u[e]);
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int k = grp + 16 * n;
+    if (k < K) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[n][e] = fmaf(kk[n], u[e], S[n][e]);
+      float* p = S0 + (int64_t)k * V + v0;
+      if (whole) store_pack<float, 4>(p, S[n]);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v0 + e < V) p[e] = S[n][e];
+    }
+  }
+  if (grp == 0) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 16; ++i) s += at4(&red[1][i][c]);
+    T* op = o + b * cfg.o_stride[0] + h * cfg.o_stride[2] + v0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (v0 + e < V) op[e] = (T)(cfg.scale * fmaf(qk_sh, u[e], s[e]));
+  }
+}
+
+__global__ void delta_keep_state(const float* __restrict__ from, float* __restrict__ to, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) to[i] = from ? from[i] : 0.f;
+}
+
+int launch_delta_scan(const DeltaDims& d, bool bwd, const int32_t* lengths, const float* M1, const float* M2, float* UT, float* ST, const float* gC,
+                      const float* first, float* last, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)d.B * d.H * d.VT));
+#define OPE_SCAN(KT)                                                                                                               \
+  case KT:                                                                                                                         \
+    if (bwd) OPE_LAUNCH((delta_scan<KT, true>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, first, last);               \
+    else OPE_LAUNCH((delta_scan<KT, false>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, first, last);                  \
+    break
+  switch (d.KT) { OPE_SCAN(1); OPE_SCAN(2); OPE_SCAN(4); OPE_SCAN(8); }
+#undef OPE_SCAN
+  OPE_CHECK_LAUNCH();
+  return OPE_OK;
+}
+
+}  // namespace ope
+using namespace ope;
+
+// floats of each array, in the order the header of ope_delta.h names them
+static void saved_layout(const DeltaDims& d, int64_t* st, int64_t* ut, int64_t* wt, int64_t* gc, int64_t* end) {
+  *st = 0;
+  *ut = *st + d.chunks * d.Vp * d.Kp;
+  *wt = *ut + d.chunks * d.Vp * kC;
+  *gc = *wt + d.chunks * d.Kp * kC;
+  *end = *gc + ((d.chunks + 3) & ~(int64_t)3);
+}
+
+extern "C" int64_t ope_delta_saved_bytes(const ope_delta_cfg* cfg) {
+  if (!delta_ok(cfg)) return OPE_EINVAL;
+  int64_t a, b, c, e, end;
+  saved_layout(delta_dims(cfg), &a, &b, &c, &e, &end);
+  return end * 4;
+}
+
+namespace ope {
+void delta_saved(const DeltaDims& d, float* saved, float** ST, float** UT, float** WT, float** gC) {
+  int64_t a, b, c, e, end;
+  saved_layout(d, &a, &b, &c, &e, &end);
+  *ST = saved + a; *UT = saved + b; *WT = saved + c; *gC = saved + e;
+}
+int64_t delta_bwd_floats(const DeltaDims& d) {
+  return d.chunks * ((int64_t)kC * d.Kp + (int64_t)d.Vp * kC + (int64_t)d.Vp * d.Kp) + (d.H != d.Hk ? 2 * (int64_t)d.B * d.T * d.H * d.K : 0);
+}
+}
+
+extern "C" int64_t ope_delta_workspace_bytes(const ope_delta_cfg* cfg, int32_t backward) {
+  if (!delta_ok(cfg)) return OPE_EINVAL;
+  const DeltaDims d = delta_dims(cfg);
+  return 4 * (backward ? delta_bwd_floats(d) : d.chunks * 2 * kC * d.Kp);
+}
+
+extern "C" int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta,
+                                 const float* state0, const int32_t* lengths, void* o, float* state_out, void* saved, int64_t saved_bytes,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!delta_ok(cfg)) return OPE_EINVAL;
+  const DeltaDims d = delta_dims(cfg);
+  hipStream_t st = (hipStream_t)stream;
+  if (d.B == 0) return OPE_OK;
+  if (!state_out) return OPE_EINVAL;
+  if (d.T == 0) {
+    const int64_t n = (int64_t)d.B * d.H * d.K * d.V;
+    OPE_LAUNCH(delta_keep_state, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, state0, state_out, n);
+    OPE_CHECK_LAUNCH();
+    return OPE_OK;
+  }
+  if (!q || !k || !v || !g || !beta || !o || !saved || !workspace) return OPE_EINVAL;
+  if (saved_bytes < ope_delta_saved_bytes(cfg) || workspace_bytes < ope_delta_workspace_bytes(cfg, 0)) return OPE_ENOSPC;
+  float *ST, *UT, *WT, *gC;
+  delta_saved(d, (float*)saved, &ST, &UT, &WT, &gC);
+  float *W = (float*)workspace, *KdT = W + d.chunks * kC * d.Kp;
+  return with_elem(cfg->dtype, [&](auto t) {
+    typedef decltype(t) T;
+    const dim3 grid((unsigned)d.chunks);
+#define OPE_PREP(KT) \
+  case KT: OPE_LAUNCH((delta_prep<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)k, (const T*)v, g, beta, lengths, W, WT, KdT, UT, gC); break
+    switch (d.KT) { OPE_PREP(1); OPE_PREP(2); OPE_PREP(4); OPE_PREP(8); }
+#undef OPE_PREP
+    OPE_CHECK_LAUNCH();
+    const int rc = launch_delta_scan(d, false, lengths, W, KdT, UT, ST, gC, state0, state_out, st);
+    if (rc) return rc;
+#define OPE_OUT(KT) \
+  case KT: OPE_LAUNCH((delta_out<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, ST, UT, (T*)o); break
+    switch (d.KT) { OPE_OUT(1); OPE_OUT(2); OPE_OUT(4); OPE_OUT(8); }
+#undef OPE_OUT
+    OPE_CHECK_LAUNCH();
+    return OPE_OK;
+  });
+}
+
+extern "C" int ope_delta_step(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
+                              void* o, void* stream) {
+  if (!delta_ok(cfg)) return OPE_EINVAL;
+  if (cfg->batch == 0) return OPE_OK;
+  if (!q || !k || !v || !g || !beta || !state || !o) return OPE_EINVAL;
+  const int64_t blocks = (int64_t)cfg->batch * cfg->n_heads * ope_cdiv(cfg->value_dim, 64);
+  if (blocks >= ((int64_t)1 << 31)) return OPE_EINVAL;
+  return with_elem(cfg->dtype, [&](auto t) {
+    typedef decltype(t) T;
+#define OPE_STEP(NK) \
+  OPE_LAUNCH((delta_step<T, NK>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *cfg, (const T*)q, (const T*)k, (const T*)v, g, beta, state, (T*)o)
+    if (cfg->key_dim <= 16) OPE_STEP(1);
+    else if (cfg->key_dim <= 32) OPE_STEP(2);
+    else if (cfg->key_dim <= 64) OPE_STEP(4);
+    else OPE_STEP(8);
+#undef OPE_STEP
+    OPE_CHECK_LAUNCH();
+    return OPE_OK;
+  });
+}
