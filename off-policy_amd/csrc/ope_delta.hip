@@ -231,28 +231,26 @@ __global__ __launch_bounds__(256) void delta_step(ope_delta_cfg cfg, const T* __
   f32x4 S[NK], sk = {0.f, 0.f, 0.f, 0.f}, sq = sk;
   float kk[NK], qk = 0.f;
   const bool whole = v0 + 4 <= V;
+  if (whole) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) S[n] = load_pack<float, 4>(S0 + (int64_t)min(grp + 16 * n, K - 1) * V + v0);
+  } else {
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[n][e] = v0 + e < V ? S0[(int64_t)min(grp + 16 * n, K - 1) * V + v0 + e] : 0.f;
+  }
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
-    const int k = grp + 16 * n;
-    S[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    kk[n] = 0.f;
-    if (k < K) {
-      const float* p = S0 + (int64_t)k * V + v0;
-      if (whole) S[n] = load_pack<float, 4>(p);
-      else
+    const int k = grp + 16 * n, kc = min(k, K - 1);      // keys past the last one: read again, weighted with 0 and not written
+    kk[n] = k < K ? (float)kp[kc] : 0.f;
+    const float qq = k < K ? (float)qp[kc] : 0.f;
+    qk = fmaf(qq, kk[n], qk);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v0 + e < V) S[n][e] = p[e];
-      if (a == 0.f) S[n] = f32x4{0.f, 0.f, 0.f, 0.f};      // a reset forgets whatever the state holds
-      else S[n] *= a;
-      kk[n] = (float)kp[k];
-      const float qq = (float)qp[k];
-      qk = fmaf(qq, kk[n], qk);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sk[e] = fmaf(S[n][e], kk[n], sk[e]);
-        sq[e] = fmaf(S[n][e], qq, sq[e]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      S[n][e] = a == 0.f || k >= K ? 0.f : S[n][e] * a;   // (a reset forgets whatever the state holds)
+      sk[e] = fmaf(S[n][e], kk[n], sk[e]);
+      sq[e] = fmaf(S[n][e], qq, sq[e]);
     }
   }
   put4(&red[0][grp][c], sk);
@@ -272,18 +270,19 @@ __global__ __launch_bounds__(256) void delta_step(ope_delta_cfg cfg, const T* __
   for (int e = 0; e < 4; ++e)
     if (v0 + e < V) u[e] = beta * ((float)v_in[b * cfg.v_stride[0] + h * cfg.v_stride[2] + v0 + e] - u[e]);
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int k = grp + 16 * n;
-    if (k < K) {
+  for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) S[n][e] = fmaf(kk[n], u[e], S[n][e]);
-      float* p = S0 + (int64_t)k * V + v0;
-      if (whole) store_pack<float, 4>(p, S[n]);
-      else
+    for (int e = 0; e < 4; ++e) S[n][e] = fmaf(kk[n], u[e], S[n][e]);
+  if (whole) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v0 + e < V) p[e] = S[n][e];
-    }
+    for (int n = 0; n < NK; ++n)
+      if (grp + 16 * n < K) store_pack<float, 4>(S0 + (int64_t)(grp + 16 * n) * V + v0, S[n]);
+  } else {
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (grp + 16 * n < K && v0 + e < V) S0[(int64_t)(grp + 16 * n) * V + v0 + e] = S[n][e];
   }
   if (grp == 0) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};

@@ -1,4 +1,8 @@
-"""What the operators' bindings share: type codes, argument checks, the raw stream and the device guard."""
+"""What the operators' bindings share: type codes, argument checks, the raw stream and the device guard.
+
+An agent acts one step at a time, so the host's share of a small call counts as much as the kernel's: what follows from sizes, strides and types
+alone (the checks, the packed configuration, the workspaces' sizes) is worked out once for each combination and kept in an lru_cache; nothing
+that depends on a tensor's place or contents is."""
 import contextlib
 
 import torch
@@ -7,34 +11,45 @@ from .. import _lib
 
 DTYPES = {torch.float32: _lib.OPE_F32, torch.bfloat16: _lib.OPE_BF16, torch.float16: _lib.OPE_F16}
 E4M3 = torch.float8_e4m3fn
+PLANS = 1024              # combinations of sizes and strides that are remembered for each entry point
 _NONE = contextlib.nullcontext()
+grad_enabled = torch.is_grad_enabled
+stream = _lib.current_stream
 
 
-def dtype_code(t, name):
-    code = DTYPES.get(t.dtype)
+def dtype_code(dtype, name):
+    code = DTYPES.get(dtype)
     if code is None:
-        raise TypeError("%s: float32, bfloat16 or float16 wanted, got %s" % (name, t.dtype))
+        raise TypeError("%s: float32, bfloat16 or float16 wanted, got %s" % (name, dtype))
     return code
 
 
-def want(t, name, shape=None, dtype=None):
-    """`t` is a tensor of that shape and type (None = not checked)."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError("%s: a tensor wanted, got %s" % (name, type(t).__name__))
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError("%s: shape %s wanted, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError("%s: %s wanted, got %s" % (name, dtype, t.dtype))
+def tensors(*named):
+    """Every (tensor, name) holds a tensor."""
+    for t, name in named:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s: a tensor wanted, got %s" % (name, type(t).__name__))
+
+
+def same_shape(shape, name, wanted):
+    if tuple(shape) != tuple(wanted):
+        raise ValueError("%s: shape %s wanted, got %s" % (name, tuple(wanted), tuple(shape)))
+
+
+def same_dtype(dtype, name, wanted):
+    if dtype != wanted:
+        raise TypeError("%s: %s wanted, got %s" % (name, wanted, dtype))
 
 
 def on_device(first, *others):
     """All tensors live on one GPU; returns a context that makes it the current device (and costs nothing where it already is)."""
-    if not first.is_cuda:
+    d = first.get_device()
+    if d < 0:
         raise ValueError("the operators run on the GPU only: got a tensor on %s" % first.device)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
             raise ValueError("tensors on %s and %s in one call" % (first.device, t.device))
-    return _NONE if torch.cuda.current_device() == first.device.index else torch.cuda.device(first.device)
+    return _NONE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)
 
 
 def inner(t):
@@ -43,9 +58,12 @@ def inner(t):
 
 
 def rows_of(t, width):
-    """`t` [..., width] as rows [n, width] at one stride, without a copy where its layout allows it. A stride below the width (an expanded
-    axis) is fine for what is only read."""
-    return inner(t.reshape(-1, width))
+    """`t` [..., width] as rows at one stride, and that stride; a copy only where the layout has none. A stride below the width (an expanded axis)
+    is fine for what is only read."""
+    if t.is_contiguous():
+        return t, width
+    t = inner(t.reshape(-1, width))
+    return t, t.stride(0)
 
 
 def like(t):
@@ -54,19 +72,27 @@ def like(t):
     return out if out.shape[-1] <= 1 or out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def stream():
-    return _lib.current_stream()
+def wants_grad(*ts):
+    if grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def scratch(nbytes, device, what):
-    """Workspace of a call (None where it needs none); a negative size is the library's refusal of the configuration."""
+def size_or_raise(nbytes, what):
+    """A negative size is the library's refusal of the configuration."""
     if nbytes < 0:
         _lib.check(nbytes, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return nbytes
+
+
+def scratch(nbytes, device):
+    """Workspace of a call: (tensor, address, size); the tensor is held until the call has been enqueued."""
+    if not nbytes:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), nbytes
 
 
 def ptr(t):

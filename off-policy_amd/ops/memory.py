@@ -1,66 +1,89 @@
 """Gated delta rule: a state matrix per head as an agent's memory, chunked over whole episodes or one step at a time (ope_delta_*)."""
+import functools
 import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._common import DTYPES, dtype_code, inner, like, on_device, ptr, scratch, stream, want, wants_grad
+from ._common import PLANS, dtype_code, inner, like, on_device, ptr, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
 
 _CFG = struct.Struct("7if33q")
 _NONE3 = (0, 0, 0)
 MAX_KEY, MAX_VALUE = 128, 1024
+_lib_forward, _lib_backward, _lib_step = _lib.lib.ope_delta_forward, _lib.lib.ope_delta_backward, _lib.lib.ope_delta_step
 
 
-def _check(q, k, v, log_decay, beta, scale, lead):
-    """`lead` axes in front of the heads (2: batch and time, 1: batch)."""
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        want(t, name)
-    code = dtype_code(q, "q")
-    if q.dim() != lead + 2 or v.dim() != lead + 2 or v.shape[:lead] != q.shape[:lead]:
-        raise ValueError("q and v: %d axes with the same first %d wanted, got %s and %s" % (lead + 2, lead, tuple(q.shape), tuple(v.shape)))
-    want(k, "k", q.shape, q.dtype)
-    want(v, "v", None, q.dtype)
-    Hk, K, H, V = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+@functools.lru_cache(PLANS)
+def _plan(q, k, v, g, beta, state, lengths, dtypes, lead):
+    """(B, T, H, Hk, K, V, type code) of shapes and types that fit together; `lead` axes in front of the heads (2: batch and time, 1: batch)."""
+    q_dtype, k_dtype, v_dtype, g_dtype, beta_dtype, state_dtype, lengths_dtype = dtypes
+    code = dtype_code(q_dtype, "q")
+    if len(q) != lead + 2 or len(v) != lead + 2 or v[:lead] != q[:lead]:
+        raise ValueError("q and v: %d axes with the same first %d wanted, got %s and %s" % (lead + 2, lead, tuple(q), tuple(v)))
+    same_shape(k, "k", q)
+    same_dtype(k_dtype, "k", q_dtype)
+    same_dtype(v_dtype, "v", q_dtype)
+    Hk, K, H, V = q[-2], q[-1], v[-2], v[-1]
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError("the value heads (%d) have to be a multiple of the query / key heads (%d)" % (H, Hk))
     if not 1 <= K <= MAX_KEY or not 1 <= V <= MAX_VALUE:
         raise ValueError("key widths of 1 to %d and value widths of 1 to %d wanted, got %d and %d" % (MAX_KEY, MAX_VALUE, K, V))
-    want(log_decay, "log_decay", v.shape[:-1], torch.float32)
-    want(beta, "beta", v.shape[:-1], torch.float32)
-    return code, float(K ** -0.5 if scale is None else scale)
+    same_shape(g, "log_decay", v[:-1])
+    same_dtype(g_dtype, "log_decay", torch.float32)
+    same_shape(beta, "beta", v[:-1])
+    same_dtype(beta_dtype, "beta", torch.float32)
+    if state is not None:
+        same_shape(state, "the state", (q[0], H, K, V))
+        same_dtype(state_dtype, "the state", torch.float32)
+    if lengths is not None:
+        same_shape(lengths, "lengths", q[:1])
+        same_dtype(lengths_dtype, "lengths", torch.int32)
+    return q[0], q[1] if lead == 2 else 1, H, Hk, K, V, code
 
 
-def _strides(*tensors):
-    out = []
-    for t in tensors:
-        out += _NONE3 if t is None else t.stride()[:3]
-    return out
+def _check(q, k, v, g, beta, state, lengths, lead):
+    tensors((q, "q"), (k, "k"), (v, "v"), (g, "log_decay"), (beta, "beta"))
+    s = s_dtype = n = n_dtype = None
+    if state is not None:
+        tensors((state, "the state"))
+        s, s_dtype = state.shape, state.dtype
+    if lengths is not None:
+        tensors((lengths, "lengths"))
+        n, n_dtype = lengths.shape, lengths.dtype
+    return _plan(q.shape, k.shape, v.shape, g.shape, beta.shape, s, n, (q.dtype, k.dtype, v.dtype, g.dtype, beta.dtype, s_dtype, n_dtype), lead)
 
 
-def _pack(shape, code, scale, q, k, v, o, g, beta, *grads):
-    """ope_delta_cfg of the call; the gradients' strides stay zero in a forward call."""
-    return _CFG.pack(*shape, code, scale, *_strides(q, k, v, o, g, beta, *(grads or (None,) * 5)))
+@functools.lru_cache(PLANS)
+def _pack(plan, scale, *strides):
+    """(configuration, bytes of `saved`, of the forward workspace, of the backward workspace); the gradients' strides are zeros in a forward call."""
+    flat = [x for s in strides for x in s[:3]]
+    cfg = _CFG.pack(*plan, scale, *flat, *(0,) * (33 - len(flat)))
+    lib, what = _lib.lib, "ope_delta"
+    return (cfg, size_or_raise(lib.ope_delta_saved_bytes(cfg), what), size_or_raise(lib.ope_delta_workspace_bytes(cfg, 0), what),
+            size_or_raise(lib.ope_delta_workspace_bytes(cfg, 1), what))
 
 
-def _forward(q, k, v, g, beta, state, lengths, scale, code):
-    (B, T, Hk, K), (H, V), dev = q.shape, v.shape[2:], q.device
+def _forward(plan, q, k, v, g, beta, state, lengths, scale):
+    B, _, H, _, K, V, _ = plan
+    dev = q.device
     o, last = like(v), torch.empty((B, H, K, V), dtype=torch.float32, device=dev)
-    cfg = _pack((B, T, H, Hk, K, V), code, scale, q, k, v, o, g, beta)
-    saved = scratch(_lib.lib.ope_delta_saved_bytes(cfg), dev, "ope_delta_forward")
-    ws = scratch(_lib.lib.ope_delta_workspace_bytes(cfg, 0), dev, "ope_delta_forward")
-    _lib.check(_lib.lib.ope_delta_forward(cfg, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(state), ptr(lengths), ptr(o), ptr(last), ptr(saved),
-                                          0 if saved is None else saved.numel(), ptr(ws), 0 if ws is None else ws.numel(), stream()), "ope_delta_forward")
+    cfg, saved_bytes, ws_bytes, _ = _pack(plan, scale, q.stride(), k.stride(), v.stride(), o.stride(), g.stride(), beta.stride())
+    saved, saved_at, _ = scratch(saved_bytes, dev)
+    hold, ws, _ = scratch(ws_bytes, dev)
+    rc = _lib_forward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), ptr(state), ptr(lengths), o.data_ptr(), last.data_ptr(),
+                      saved_at, saved_bytes, ws, ws_bytes, stream())
+    if rc:
+        _lib.check(rc, "ope_delta_forward")
     return o, last, saved
 
 
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, lengths, scale):
-        with on_device(q, k, v, g, beta, state, lengths):
-            o, last, saved = _forward(q, k, v, g, beta, state, lengths, scale, DTYPES[q.dtype])
+    def forward(ctx, q, k, v, g, beta, state, lengths, scale, plan):
+        o, last, saved = _forward(plan, q, k, v, g, beta, state, lengths, scale)
         ctx.save_for_backward(q, k, v, g, beta, lengths, saved)
-        ctx.scale = scale
+        ctx.scale, ctx.plan = scale, plan
         ctx.set_materialize_grads(False)
         return o, last
 
@@ -68,20 +91,23 @@ class _GatedDelta(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do, dlast):
         if do is None and dlast is None:
-            return (None,) * 8
+            return (None,) * 9
         q, k, v, g, beta, lengths, saved = ctx.saved_tensors
-        (B, T, Hk, K), (H, V), dev = q.shape, v.shape[2:], q.device
+        B, _, H, _, K, V, _ = plan = ctx.plan
         with on_device(q, do, dlast):
+            dev = q.device
             do = torch.zeros(v.shape, dtype=v.dtype, device=dev) if do is None else inner(do)
             dlast = None if dlast is None else dlast.contiguous()
             dq, dk, dv, dg, db = like(q), like(k), like(v), torch.empty_like(g), torch.empty_like(beta)
             dstate = torch.empty((B, H, K, V), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
-            cfg = _pack((B, T, H, Hk, K, V), DTYPES[q.dtype], ctx.scale, q, k, v, do, g, beta, dq, dk, dv, dg, db)
-            ws = scratch(_lib.lib.ope_delta_workspace_bytes(cfg, 1), dev, "ope_delta_backward")
-            _lib.check(_lib.lib.ope_delta_backward(cfg, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(lengths), ptr(saved),
-                                                   0 if saved is None else saved.numel(), ptr(do), ptr(dlast), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(db),
-                                                   ptr(dstate), ptr(ws), 0 if ws is None else ws.numel(), stream()), "ope_delta_backward")
-        return dq, dk, dv, dg, db, dstate, None, None
+            cfg, saved_bytes, _, ws_bytes = _pack(plan, ctx.scale, q.stride(), k.stride(), v.stride(), do.stride(), g.stride(), beta.stride(), dq.stride(),
+                                                  dk.stride(), dv.stride(), dg.stride(), db.stride())
+            hold, ws, _ = scratch(ws_bytes, dev)
+            rc = _lib_backward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(saved), saved_bytes, do.data_ptr(),
+                               ptr(dlast), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), db.data_ptr(), ptr(dstate), ws, ws_bytes, stream())
+            if rc:
+                _lib.check(rc, "ope_delta_backward")
+        return dq, dk, dv, dg, db, dstate, None, None, None
 
 
 def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None, scale=None):
@@ -98,38 +124,38 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
 
     Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 at -inf), beta and
     initial_state. The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32: (K V + 64 (K + V)) * 4 bytes."""
-    code, scale = _check(q, k, v, log_decay, beta, scale, 2)
-    B, K, H, V = q.shape[0], q.shape[-1], v.shape[-2], v.shape[-1]
-    if initial_state is not None:
-        want(initial_state, "initial_state", (B, H, K, V), torch.float32)
-    if lengths is not None:
-        want(lengths, "lengths", (B,), torch.int32)
-        lengths = lengths.contiguous()
-    guard = on_device(q, k, v, log_decay, beta, initial_state, lengths)
-    grads = wants_grad(q, k, v, log_decay, beta, initial_state)
-    q, k, v = inner(q), inner(k), inner(v)
-    state = None if initial_state is None else initial_state.contiguous()
-    if grads:
-        return _GatedDelta.apply(q, k, v, log_decay, beta, state, lengths, scale)
-    with guard:
-        return _forward(q, k, v, log_decay, beta, state, lengths, scale, code)[:2]
+    plan = _check(q, k, v, log_decay, beta, initial_state, lengths, 2)
+    scale = float(plan[4] ** -0.5 if scale is None else scale)
+    with on_device(q, k, v, log_decay, beta, initial_state, lengths):
+        q, k, v = inner(q), inner(k), inner(v)
+        state = None if initial_state is None else initial_state.contiguous()
+        lengths = None if lengths is None else lengths.contiguous()
+        if wants_grad(q, k, v, log_decay, beta, state):
+            return _GatedDelta.apply(q, k, v, log_decay, beta, state, lengths, scale, plan)
+        return _forward(plan, q, k, v, log_decay, beta, state, lengths, scale)[:2]
+
+
+@functools.lru_cache(PLANS)
+def _pack_step(plan, scale, q, k, v, g, beta):
+    _, _, H, _, _, V, _ = plan
+    three = lambda s: (s[0], 0, s[1])       # noqa: E731
+    return _CFG.pack(*plan, float(plan[4] ** -0.5 if scale is None else scale), *three(q), *three(k), *three(v), H * V, 0, V, *three(g), *three(beta), *_NONE3 * 5)
 
 
 def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
     """One token of gated_delta_rule for every row: q, k [B, Hk, K], v [B, H, V], log_decay, beta float32 [B, H]; `state` float32 [B, H, K, V], contiguous,
     is updated in place (log_decay = -inf: cleared first, whatever it holds). Returns out [B, H, V]. For acting: no gradients."""
-    code, scale = _check(q, k, v, log_decay, beta, scale, 1)
-    B, Hk, K = q.shape
-    H, V = v.shape[1:]
-    want(state, "state", (B, H, K, V), torch.float32)
+    tensors((state, "the state"))
+    plan = _check(q, k, v, log_decay, beta, state, None, 1)
     if not state.is_contiguous():
-        raise ValueError("state: it is updated in place and has to be contiguous")
+        raise ValueError("the state is updated in place and has to be contiguous")
     if wants_grad(q, k, v, log_decay, beta, state):
         raise ValueError("gated_delta_step has no gradients: call it under torch.no_grad(), or gated_delta_rule")
     with on_device(q, k, v, log_decay, beta, state):
         q, k, v = inner(q), inner(k), inner(v)
-        o = torch.empty((B, H, V), dtype=v.dtype, device=v.device)
-        cfg = _CFG.pack(B, 1, H, Hk, K, V, code, scale, q.stride(0), 0, q.stride(1), k.stride(0), 0, k.stride(1), v.stride(0), 0, v.stride(1), H * V, 0, V,
-                        log_decay.stride(0), 0, log_decay.stride(1), beta.stride(0), 0, beta.stride(1), *_NONE3 * 5)
-        _lib.check(_lib.lib.ope_delta_step(cfg, ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(beta), ptr(state), ptr(o), stream()), "ope_delta_step")
+        o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        rc = _lib_step(_pack_step(plan, scale, q.stride(), k.stride(), v.stride(), log_decay.stride(), beta.stride()), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                       log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), stream())
+        if rc:
+            _lib.check(rc, "ope_delta_step")
     return o
