@@ -5,12 +5,16 @@
 // its "transposed chain" (lane (j, g) holds features 4g .. 4g+3 of data row j) is both the form a product leaves and the form the next one
 // reads, so the triangular solve and the scan need no shuffles.
 //
-// Arrays in `saved` (S, kept for the backward pass) and in the workspace (W), all float32:
-//   ST  [c][Vp][Kp]   S  the state in front of the chunk, transposed          UT [c][Vp][64]  S  u of the chunk's tokens (U0 before the scan)
-//   WT  [c][Kp][64]   S  W transposed                                         gC [c]          S  decay over the whole chunk (0 behind a reset)
-//   W   [c][64][Kp]   W                                                       KdT [c][Kp][64] W  k_t * decay from t to the chunk's end
-//   backward: Kd [c][64][Kp], dUT [c][Vp][64] (dU0, then dU, then dR), dST [c][Vp][Kp] (N, then the gradient of the state BEHIND the chunk),
-//   dqp, dkp [b][t][H][K] where query / key heads are shared
+// Arrays in `saved` (S, kept for the backward pass) and in the workspace (W). All lie in TILES of 16 x 16, in the order in which the lanes of a
+// wave hold them: lane (j, g) has row j, columns 4g .. 4g+3, tile after tile, so that every access of a wave is one run of whole cache lines (rows
+// of the matrices themselves took twice the time: a CU's requests in flight, not its bytes, bound the scan). turn4 gives a tile transposed.
+//   ST  [c][VT][KT]  float32 S  the state in front of the chunk: rows v, columns k       (a tile index is the last two indexes)
+//   UT  [c][VT][4]   float32 S  u of the chunk's tokens (U0 before the scan): rows v, columns t
+//   WT  [c][KT][4]   float32 S  W transposed: rows k, columns t
+//   gC  [c]          float32 S  decay over the whole chunk (0 behind a reset);  tails [c][64] float32 S  decay from t to the chunk's end
+//   W   [c][4][KT]   float32 W  rows t, columns k                                KTs [c][KT][4] of the inputs' type W  k transposed: rows k, columns t
+//   backward: Ks [c][4][KT] of the inputs' type W (rows t, columns k), dUT like UT (dU0, then dU, then dR), dST like ST (N, then the gradient of the
+//   state BEHIND the chunk), dqp, dkp [b][t][H][K] float32 where query / key heads are shared
 #pragma once
 #include <type_traits>
 
@@ -94,23 +98,42 @@ __device__ __forceinline__ void load_gates(Gates& s, const ope_delta_cfg& c, con
   if (t == 63) s.whole = seg == 0 ? expf((float)G) : 0.f;
 }
 
-// A chunk of q or k as float32 in LDS [64][Kp + 4]; what lies outside (tokens that are not live, columns past K) is 0. 256 threads.
+// A chunk of q or k in LDS, in its own type, rows 16 bytes longer than the padded width (16 rows read at one column then hit different banks).
 template <typename T, int KT>
-__device__ __forceinline__ void load_rows(float (*dst)[16 * KT + 4], const T* p, const int64_t* stride, const ChunkAt& a, int head, int K) {
+struct Rows {
+  static constexpr int kStride = 16 * KT + 16 / (int)sizeof(T);
+  T v[kC][kStride];
+};
+// What lies outside (tokens that are not live, columns past K) is 0.
+template <typename T, int KT>
+__device__ __forceinline__ void load_rows(Rows<T, KT>& dst, const T* p, const int64_t* stride, const ChunkAt& a, int head, int K) {
+  typedef typename Pack<T, 4>::vec vec;
   const T* base = p + a.b * stride[0] + (int64_t)a.t0 * stride[1] + head * stride[2];
-  for (int q = threadIdx.x; q < kC * KT * 4; q += 256) {
+  for (int q = threadIdx.x; q < kC * KT * 4; q += blockDim.x) {
     const int t = q / (KT * 4), k = (q % (KT * 4)) * 4;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    vec v = (vec)(T)0.f;
     if (t < a.nv) {
       const T* row = base + (int64_t)t * stride[1];
-      if (k + 4 <= K) v = load_pack<T, 4>(row + k);
+      if (k + 4 <= K) v = *reinterpret_cast<const typename Pack<T, 4>::loose*>(row + k);
       else
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (k + e < K) v[e] = (float)row[k + e];
+          if (k + e < K) v[e] = row[k + e];
     }
-    *reinterpret_cast<f32x4*>(&dst[t][k]) = v;
+    *reinterpret_cast<vec*>(&dst.v[t][k]) = v;
   }
+}
+// four elements of a row / of a column, as float32
+template <typename T>
+__device__ __forceinline__ f32x4 row4(const T* p) {
+  return __builtin_convertvector(*reinterpret_cast<const typename Pack<T, 4>::vec*>(p), f32x4);
+}
+template <typename T>
+__device__ __forceinline__ f32x4 column4(const T* p, int stride) {
+  f32x4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = (float)p[r * stride];
+  return v;
 }
 
 __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {   // 16 x 16 x 16: four steps of the f32 matrix instruction
@@ -118,8 +141,42 @@ __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {   // 16 x 16
   for (int r = 0; r < 4; ++r) c = mfma16(a[r], b[r], c);
   return c;
 }
+// The same product of two rows as they lie in LDS. Products of bfloat16 and float16 are exact in float32 and their matrix instructions add them in
+// float32 (measured: 1.8e-8 of the result's norm, as the f32 instruction), at 8 times its rate: nothing is lost by not widening first.
+__device__ __forceinline__ f32x4 dot4(const float* a, const float* b, f32x4 c) { return mfma4(row4(a), row4(b), c); }
+__device__ __forceinline__ f32x4 dot4(const bf16_t* a, const bf16_t* b, f32x4 c) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(*reinterpret_cast<const s16x4*>(a), *reinterpret_cast<const s16x4*>(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 dot4(const f16_t* a, const f16_t* b, f32x4 c) {
+  typedef Pack<f16_t, 4>::vec vec;
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(*reinterpret_cast<const vec*>(a), *reinterpret_cast<const vec*>(b), c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4 at4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 __device__ __forceinline__ void put4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+// A lane's place in a tile, and its place in the same tile read or written transposed (turn4 on the far side).
+__device__ __forceinline__ int tile_lane() { return (threadIdx.x & 63) * 4; }
+__device__ __forceinline__ int turned_lane() {
+  const int j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  return (4 * g + (j & 3) + 16 * (j >> 2)) * 4;
+}
+// Transpose of the 4 x 4 that four neighbouring lanes hold: result[e] = lane e's x[own place in the four].
+__device__ __forceinline__ f32x4 turn4(f32x4 x) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    const float got = OPE_DPP_F(odd ? x[e] : x[e + 1], 0xB1);
+    x[e] = odd ? got : x[e];
+    x[e + 1] = odd ? x[e + 1] : got;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float got = OPE_DPP_F(high ? x[e] : x[e + 2], 0x4E);
+    x[e] = high ? got : x[e];
+    x[e + 2] = high ? x[e + 2] : got;
+  }
+  return x;
+}
 __device__ __forceinline__ f32x4 col4(const float* p, int64_t stride) {   // four elements `stride` apart
   f32x4 v;
 #pragma unroll
@@ -127,20 +184,27 @@ __device__ __forceinline__ f32x4 col4(const float* p, int64_t stride) {   // fou
   return v;
 }
 
-// -A (strictly lower, -A_ij = -beta_i decay(i, j) k_i.k_j) of the chunk in LDS, zero elsewhere. 4 waves, one row of tiles each; barrier behind.
-template <int KT>
-__device__ __forceinline__ void minus_A(float (*NA)[kC + 4], const float (*k)[16 * KT + 4], const Gates& gt) {
-  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-  const int t = 16 * w + j;
-  for (int is = 0; is < 4; ++is) {
+// tile x of the 10 on and below the diagonal of a chunk's 4 x 4
+__device__ __forceinline__ void lower_tile(int x, int& it, int& is) {
+  it = x < 1 ? 0 : (x < 3 ? 1 : (x < 6 ? 2 : 3));
+  is = x - it * (it + 1) / 2;
+}
+// -A (strictly lower, -A_ij = -beta_i decay(i, j) k_i.k_j) of the chunk in LDS: the 10 tiles on and below the diagonal, zeros above it in the
+// diagonal tiles (the tiles above are neither written nor read). Tiles are dealt out to the waves; barrier behind.
+template <typename T, int KT>
+__device__ __forceinline__ void minus_A(float (*NA)[kC + 4], const Rows<T, KT>& k, const Gates& gt) {
+  const int j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  for (int x = threadIdx.x >> 6; x < 10; x += blockDim.x >> 6) {
+    int it, is;
+    lower_tile(x, it, is);
+    const int t = 16 * it + j;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (is <= w) {
-      for (int c = 0; c < KT; ++c) acc = mfma4(at4(&k[16 * is + j][16 * c + 4 * g]), at4(&k[t][16 * c + 4 * g]), acc);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int s = 16 * is + 4 * g + r;
-        acc[r] = s < t ? -gt.beta[t] * decay(gt, t, s) * acc[r] : 0.f;
-      }
+    for (int c = 0; c < KT; ++c) acc = dot4(&k.v[16 * is + j][16 * c + 4 * g], &k.v[t][16 * c + 4 * g], acc);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int s = 16 * is + 4 * g + r;
+      acc[r] = s < t ? -gt.beta[t] * decay(gt, t, s) * acc[r] : 0.f;
     }
     put4(&NA[t][16 * is + 4 * g], acc);
   }
@@ -164,5 +228,9 @@ __device__ __forceinline__ void diag_inverse(float (*inv)[16][20], const float (
     inv[blk][i][c] = v;
   }
 }
+
+// waves of a workgroup in the kernels that work on whole chunks: 4, or 8 where the keys are wide enough to keep them busy
+template <int KT>
+constexpr int chunk_waves() { return KT >= 4 ? 8 : 4; }
 
 }  // namespace ope

@@ -17,44 +17,50 @@ bool delta_ok(const ope_delta_cfg* c) {
 
 // Rows of one chunk-head: W = (I + A)^-1 beta e^G k, U0 = (I + A)^-1 beta v by block forward substitution, 16 columns a wave at a time.
 template <typename T, int KT>
-__global__ __launch_bounds__(256) void delta_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ k_in, const T* __restrict__ v_in,
-                                                  const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
-                                                  float* __restrict__ W, float* __restrict__ WT, float* __restrict__ KdT, float* __restrict__ UT,
-                                                  float* __restrict__ gC) {
-  constexpr int Kp = 16 * KT;
-  __shared__ float k[kC][Kp + 4], NA[kC][kC + 4], inv[4][16][20];
+__global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ k_in, const T* __restrict__ v_in,
+                                                                    const float* __restrict__ g_in, const float* __restrict__ beta_in,
+                                                                    const int32_t* __restrict__ lengths, float* __restrict__ W, float* __restrict__ WT,
+                                                                    T* __restrict__ KTs, float* __restrict__ UT, float* __restrict__ gC,
+                                                                    float* __restrict__ tails) {
+  constexpr int NW = chunk_waves<KT>();
+  __shared__ Rows<T, KT> k;
+  __shared__ float NA[kC][kC + 4], inv[4][16][20];
   __shared__ Gates gt;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
   if (a.nv == 0) return;
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
-  load_rows<T, KT>(k, k_in, cfg.k_stride, a, a.h / (d.H / d.Hk), d.K);
+  load_rows(k, k_in, cfg.k_stride, a, a.h / (d.H / d.Hk), d.K);
   __syncthreads();
-  minus_A<KT>(NA, k, gt);
+  minus_A<T, KT>(NA, k, gt);
   if (threadIdx.x == 0) gC[a.c] = gt.whole;
+  if (threadIdx.x < kC) tails[a.c * kC + threadIdx.x] = gt.tail[threadIdx.x];
   __syncthreads();
   if (w == 0) diag_inverse(inv, NA);
-  for (int q = threadIdx.x; q < Kp * 16; q += 256) {     // KdT: four tokens of one feature a thread
-    const int f = q / 16, t = (q % 16) * 4;
-    f32x4 v;
+  for (int x = w; x < 4 * KT; x += NW) {                 // k transposed, a tile a wave
+    const int kt = x >> 2, it = x & 3;
+    typename Pack<T, 4>::vec v;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = k[t + r][f] * gt.tail[t + r];
-    put4(&KdT[(a.c * Kp + f) * kC + t], v);
+    for (int r = 0; r < 4; ++r) v[r] = k.v[16 * it + 4 * g + r][16 * kt + j];
+    *reinterpret_cast<typename Pack<T, 4>::vec*>(KTs + (a.c * KT * 4 + x) * 256 + tile_lane()) = v;
   }
   __syncthreads();
   const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)a.t0 * cfg.v_stride[1] + a.h * cfg.v_stride[2];
-  for (int cg = w; cg < KT + d.VT; cg += 4) {
+  for (int cg = w; cg < KT + d.VT; cg += NW) {
     f32x4 x[4];
     const int col = cg < KT ? 16 * cg + j : 16 * (cg - KT) + j;
+    if (cg < KT) {
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
+      for (int it = 0; it < 4; ++it) x[it] = column4(&k.v[16 * it + 4 * g][col], Rows<T, KT>::kStride) * at4(&gt.head[16 * it + 4 * g]) * at4(&gt.beta[16 * it + 4 * g]);
+    } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * it + 4 * g + r;
-        float v = 0.f;
-        if (cg < KT) v = gt.head[t] * k[t][col];
-        else if (t < a.nv && col < d.V) v = (float)v0[(int64_t)t * cfg.v_stride[1] + col];
-        x[it][r] = gt.beta[t] * v;
+      for (int it = 0; it < 4; ++it) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = 16 * it + 4 * g + r;
+          x[it][r] = t < a.nv && col < d.V ? (float)v0[(int64_t)t * cfg.v_stride[1] + col] : 0.f;
+        }
+        x[it] *= at4(&gt.beta[16 * it + 4 * g]);
       }
     }
 #pragma unroll
@@ -64,11 +70,10 @@ __global__ __launch_bounds__(256) void delta_prep(ope_delta_cfg cfg, DeltaDims d
       for (int kt = 0; kt < it; ++kt) acc = mfma4(at4(&NA[16 * it + j][16 * kt + 4 * g]), x[kt], acc);
       x[it] = mfma4(at4(&inv[it][j][4 * g]), acc, f32x4{0.f, 0.f, 0.f, 0.f});
       if (cg < KT) {
-        put4(&WT[(a.c * Kp + col) * kC + 16 * it + 4 * g], x[it]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) W[(a.c * kC + 16 * it + 4 * g + r) * Kp + col] = x[it][r];
+        put4(&WT[((a.c * KT + cg) * 4 + it) * 256 + tile_lane()], x[it]);
+        put4(&W[((a.c * 4 + it) * KT + cg) * 256 + turned_lane()], turn4(x[it]));
       } else {
-        put4(&UT[(a.c * d.Vp + col) * kC + 16 * it + 4 * g], x[it]);
+        put4(&UT[((a.c * d.VT + cg - KT) * 4 + it) * 256 + tile_lane()], x[it]);
       }
     }
   }
@@ -76,19 +81,36 @@ __global__ __launch_bounds__(256) void delta_prep(ope_delta_cfg cfg, DeltaDims d
 
 // The scan, forward or backward in time. Four waves share 16 value columns of one (sequence, head): wave w makes the 16 tokens 16w.. of
 // P = M1 S (64 x Kp times Kp x 16), then its share of the state's tiles of 16 keys. S lives in registers; it and U cross between the waves
-// through LDS, two barriers a chunk. The chain of a chunk is what bounds it, so the operands of the next one are loaded a chunk ahead.
-//   forward : U = U0 - W S;     S' = gC S + KdT U            M1 = W,  M2 = KdT
-//   backward: dU = dU0 + Kd dS'; dS = gC dS' + N - WT dU      M1 = Kd, M2 = WT
-template <int KT, bool BWD>
-__global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __restrict__ lengths, const float* __restrict__ M1,
-                                                  const float* __restrict__ M2, float* __restrict__ UT, float* __restrict__ ST,
-                                                  const float* __restrict__ gC, const float* __restrict__ first, float* __restrict__ last) {
-  constexpr int Kp = 16 * KT, NK = (KT + 3) / 4;      // tiles of keys a wave
+// through LDS, two barriers a chunk. The chain of a chunk is what bounds it, so every chunk's operands are loaded two chunks ahead into their own
+// registers (two sets, the loop is unrolled by two).
+//   forward : U = U0 - W S;            S' = gC S + k^T (tail U)          M1 = W (float32),   M2 = KTs
+//   backward: dU = dU0 + tail (k dS'); dS = gC dS' + N - WT dU           M1 = Ks,            M2 = WT (float32)
+// (a row of tail scales a product's result or its operand: the keys themselves stay in their own type, at half the bytes.)
+template <typename T, int KT, bool BWD>
+struct ScanOperands {
+  static constexpr int NK = (KT + 3) / 4;             // tiles of keys a wave
+  typedef typename std::conditional<BWD, T, float>::type T1;
+  typedef typename std::conditional<BWD, float, T>::type T2;
+  typename Pack<T1, 4>::vec m1[KT];
+  typename Pack<T2, 4>::vec m2[NK][4];
+  f32x4 u, add[NK], tail;
+  float whole;
+};
+template <typename T, int KT, bool BWD>
+__global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __restrict__ lengths, const void* M1v, const void* M2v, float* UT, float* ST,
+                                                  const float* gC, const float* tails, const float* __restrict__ first, float* __restrict__ last) {
+  constexpr int Kp = 16 * KT, NK = (KT + 3) / 4;
+  typedef ScanOperands<T, KT, BWD> Ops;
+  const typename Ops::T1* M1 = (const typename Ops::T1*)M1v;
+  const typename Ops::T2* M2 = (const typename Ops::T2*)M2v;
   __shared__ float SL[16][Kp + 4], UL[16][kC + 4];
-  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-  const int vt = blockIdx.x % d.VT;
-  const int64_t bh = blockIdx.x / d.VT;
-  const int b = (int)(bh / d.H), v = 16 * vt + j;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  // Workgroups of one (sequence, head) read the same M1 and M2: they are dealt to one XCD (workgroup index mod 8) in whole groups of 8 heads.
+  const unsigned VT = d.VT, group = blockIdx.x / (8 * VT), in = blockIdx.x % (8 * VT);
+  const bool grouped = (group + 1) * 8ull <= (unsigned long long)d.B * d.H;
+  const int vt = grouped ? in / 8 : blockIdx.x % VT;
+  const int64_t bh = grouped ? group * 8ll + in % 8 : blockIdx.x / VT;
+  const int b = (int)(bh / d.H), v = 16 * vt + j, lane = tile_lane();
   const int n = ope_cdiv_dev(live_len(lengths, b, d.T), kC);
   f32x4 S[NK];
 #pragma unroll
@@ -98,50 +120,67 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
       const int k = 16 * (w + 4 * q) + 4 * g + r;
       S[q][r] = first && k < d.K && v < d.V ? first[(bh * d.K + k) * d.V + v] : 0.f;
     }
-  f32x4 m1[KT], m2[NK][4], u, add[NK];
-  float whole = 0.f;
-  auto fetch = [&](int i) {
-    const int64_t c = bh * d.n + i;
+  auto fetch = [&](Ops& o, int s) {       // step s of the walk; past the end: the last one again
+    const int64_t c = bh * d.n + (BWD ? n - 1 - min(s, n - 1) : min(s, n - 1));
 #pragma unroll
-    for (int q = 0; q < KT; ++q) m1[q] = at4(&M1[(c * kC + 16 * w + j) * Kp + 16 * q + 4 * g]);
-    u = at4(&UT[(c * d.Vp + v) * kC + 16 * w + 4 * g]);
+    for (int q = 0; q < KT; ++q) o.m1[q] = *reinterpret_cast<const decltype(o.m1[0] + o.m1[0])*>(M1 + ((c * 4 + w) * KT + q) * 256 + lane);
+    o.u = at4(&UT[((c * VT + vt) * 4 + w) * 256 + lane]);
 #pragma unroll
-    for (int q = 0; q < NK; ++q)
-      if (w + 4 * q < KT) {
+    for (int q = 0; q < NK; ++q) {
+      const int kt = min(w + 4 * q, KT - 1);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) m2[q][p] = at4(&M2[(c * Kp + 16 * (w + 4 * q) + j) * kC + 16 * p + 4 * g]);
-        if (BWD) add[q] = at4(&ST[(c * d.Vp + v) * Kp + 16 * (w + 4 * q) + 4 * g]);
-      }
-    whole = gC[c];
+      for (int p = 0; p < 4; ++p) o.m2[q][p] = *reinterpret_cast<const decltype(o.m2[0][0] + o.m2[0][0])*>(M2 + ((c * KT + kt) * 4 + p) * 256 + lane);
+      if (BWD) o.add[q] = at4(&ST[((c * VT + vt) * KT + kt) * 256 + lane]);
+    }
+    o.tail = at4(&tails[c * kC + 16 * w + 4 * g]);
+    o.whole = gC[c];
   };
-  if (n > 0) fetch(BWD ? n - 1 : 0);
-  for (int s = 0; s < n; ++s) {
-    const int i = BWD ? n - 1 - s : s;
-    const int64_t c = bh * d.n + i;
+  auto step = [&](Ops& o, int s) {
+    const int64_t c = bh * d.n + (BWD ? n - 1 - s : s);
 #pragma unroll
     for (int q = 0; q < NK; ++q)
-      if (w + 4 * q < KT) {
-        const int k = 16 * (w + 4 * q) + 4 * g;
-        put4(&SL[j][k], S[q]);
-        put4(&ST[(c * d.Vp + v) * Kp + k], S[q]);
+      if (KT % 4 == 0 || w + 4 * q < KT) {
+        put4(&SL[j][16 * (w + 4 * q) + 4 * g], S[q]);
+        put4(&ST[((c * VT + vt) * KT + w + 4 * q) * 256 + lane], S[q]);
       }
     lds_barrier();
-    f32x4 p0 = {0.f, 0.f, 0.f, 0.f};
+    f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
 #pragma unroll
-    for (int q = 0; q < KT; ++q) p0 = mfma4(m1[q], at4(&SL[j][16 * q + 4 * g]), p0);
-    u = BWD ? u + p0 : u - p0;
-    put4(&UL[j][16 * w + 4 * g], u);
-    put4(&UT[(c * d.Vp + v) * kC + 16 * w + 4 * g], u);
+    for (int q = 0; q < KT; ++q) {
+      f32x4& p = q & 1 ? p1 : p0;
+      p = mfma4(__builtin_convertvector(o.m1[q], f32x4), at4(&SL[j][16 * q + 4 * g]), p);
+    }
+    const f32x4 u = BWD ? o.u + o.tail * (p0 + p1) : o.u - (p0 + p1);
+    put4(&UL[j][16 * w + 4 * g], BWD ? u : u * o.tail);
+    put4(&UT[((c * VT + vt) * 4 + w) * 256 + lane], u);
     lds_barrier();
 #pragma unroll
     for (int q = 0; q < NK; ++q)
-      if (w + 4 * q < KT) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      if (KT % 4 == 0 || w + 4 * q < KT) {
+        f32x4 a0 = {0.f, 0.f, 0.f, 0.f}, a1 = a0;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) acc = mfma4(m2[q][p], at4(&UL[j][16 * p + 4 * g]), acc);
-        S[q] = BWD ? whole * S[q] + add[q] - acc : whole * S[q] + acc;
+        for (int p = 0; p < 4; ++p) {
+          f32x4& x = p & 1 ? a1 : a0;
+          x = mfma4(__builtin_convertvector(o.m2[q][p], f32x4), at4(&UL[j][16 * p + 4 * g]), x);
+        }
+        S[q] = BWD ? o.whole * S[q] + o.add[q] - (a0 + a1) : o.whole * S[q] + (a0 + a1);
       }
-    if (s + 1 < n) fetch(BWD ? n - 2 - s : s + 1);
+    // Here and no earlier: hoisted above the products (the compiler's own wish) these loads need registers of their own, and the copies into the
+    // loop's wait for them at once. (M1, M2 are not __restrict__ for the same reason.)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    fetch(o, s + 2);
+  };
+  if (n > 0) {
+    Ops even, odd;
+    fetch(even, 0);
+    fetch(odd, 1);
+    int s = 0;
+    for (; s + 1 < n; s += 2) {
+      step(even, s);
+      step(odd, s + 1);
+    }
+    if (s < n) step(even, s);
   }
 #pragma unroll
   for (int q = 0; q < NK; ++q)
@@ -153,13 +192,12 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
 }
 
 // o of one chunk-head. Wave w owns the tokens 16w..: its rows of scale tril(q k^T decay) and of scale e^G q stay in registers while it walks
-// the value columns.
+// the value columns; S and U of the next 16 columns are loaded while these are multiplied.
 template <typename T, int KT>
-__global__ __launch_bounds__(256) void delta_out(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
+__global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
                                                  const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
                                                  const float* __restrict__ ST, const float* __restrict__ UT, T* __restrict__ o) {
-  constexpr int Kp = 16 * KT;
-  __shared__ float q[kC][Kp + 4], k[kC][Kp + 4];
+  __shared__ Rows<T, KT> k, q;
   __shared__ Gates gt;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -169,21 +207,28 @@ __global__ __launch_bounds__(256) void delta_out(ope_delta_cfg cfg, DeltaDims d,
     for (int e = threadIdx.x; e < rows * d.V; e += 256) o0[(int64_t)(e / d.V) * cfg.o_stride[1] + e % d.V] = (T)0.f;
     return;
   }
+  f32x4 s0[KT], u0[4];
+  auto fetch = [&](int vt) {
+    const int64_t at = a.c * d.VT + vt;
+#pragma unroll
+    for (int c = 0; c < KT; ++c) s0[c] = at4(&ST[(at * KT + c) * 256 + tile_lane()]);
+#pragma unroll
+    for (int is = 0; is < 4; ++is) u0[is] = at4(&UT[(at * 4 + min(is, w)) * 256 + tile_lane()]);
+  };
+  fetch(0);
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
   const int hk = a.h / (d.H / d.Hk);
-  load_rows<T, KT>(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows<T, KT>(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
   const int t = 16 * w + j;
   f32x4 qs[KT], P[4];
-#pragma unroll
-  for (int c = 0; c < KT; ++c) qs[c] = at4(&q[t][16 * c + 4 * g]);
 #pragma unroll
   for (int is = 0; is < 4; ++is) {
     P[is] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (is <= w) {
 #pragma unroll
-      for (int c = 0; c < KT; ++c) P[is] = mfma4(at4(&k[16 * is + j][16 * c + 4 * g]), qs[c], P[is]);
+      for (int c = 0; c < KT; ++c) P[is] = dot4(&k.v[16 * is + j][16 * c + 4 * g], &q.v[t][16 * c + 4 * g], P[is]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int s = 16 * is + 4 * g + r;
@@ -193,15 +238,22 @@ __global__ __launch_bounds__(256) void delta_out(ope_delta_cfg cfg, DeltaDims d,
   }
   const float f = cfg.scale * gt.head[t];
 #pragma unroll
-  for (int c = 0; c < KT; ++c) qs[c] *= f;
+  for (int c = 0; c < KT; ++c) qs[c] = row4(&q.v[t][16 * c + 4 * g]) * f;
   for (int vt = 0; vt < d.VT; ++vt) {
     const int v = 16 * vt + j;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4 s1[KT], u1[4];
 #pragma unroll
-    for (int c = 0; c < KT; ++c) acc = mfma4(qs[c], at4(&ST[(a.c * d.Vp + v) * Kp + 16 * c + 4 * g]), acc);
+    for (int c = 0; c < KT; ++c) s1[c] = s0[c];
+#pragma unroll
+    for (int is = 0; is < 4; ++is) u1[is] = u0[is];
+    if (vt + 1 < d.VT) fetch(vt + 1);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
+#pragma unroll
+    for (int c = 0; c < KT; ++c) acc = mfma4(qs[c], s1[c], acc);
 #pragma unroll
     for (int is = 0; is < 4; ++is)
-      if (is <= w) acc = mfma4(P[is], at4(&UT[(a.c * d.Vp + v) * kC + 16 * is + 4 * g]), acc);
+      if (is <= w) acc2 = mfma4(P[is], u1[is], acc2);
+    acc += acc2;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int tt = 16 * w + 4 * g + r;
@@ -299,48 +351,42 @@ __global__ void delta_keep_state(const float* __restrict__ from, float* __restri
   if (i < n) to[i] = from ? from[i] : 0.f;
 }
 
-int launch_delta_scan(const DeltaDims& d, bool bwd, const int32_t* lengths, const float* M1, const float* M2, float* UT, float* ST, const float* gC,
-                      const float* first, float* last, hipStream_t st) {
+int launch_delta_scan(int dtype, const DeltaDims& d, bool bwd, const int32_t* lengths, const void* M1, const void* M2, float* UT, float* ST,
+                      const float* gC, const float* tails, const float* first, float* last, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)d.B * d.H * d.VT));
+  return with_elem(dtype, [&](auto t) {
+    typedef decltype(t) T;
 #define OPE_SCAN(KT)                                                                                                               \
   case KT:                                                                                                                         \
-    if (bwd) OPE_LAUNCH((delta_scan<KT, true>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, first, last);               \
-    else OPE_LAUNCH((delta_scan<KT, false>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, first, last);                  \
+    if (bwd) OPE_LAUNCH((delta_scan<T, KT, true>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, tails, first, last);     \
+    else OPE_LAUNCH((delta_scan<T, KT, false>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, tails, first, last);        \
     break
-  switch (d.KT) { OPE_SCAN(1); OPE_SCAN(2); OPE_SCAN(4); OPE_SCAN(8); }
+    switch (d.KT) { OPE_SCAN(1); OPE_SCAN(2); OPE_SCAN(4); OPE_SCAN(8); }
 #undef OPE_SCAN
-  OPE_CHECK_LAUNCH();
-  return OPE_OK;
+    OPE_CHECK_LAUNCH();
+    return OPE_OK;
+  });
 }
 
 }  // namespace ope
 using namespace ope;
 
-// floats of each array, in the order the header of ope_delta.h names them
-static void saved_layout(const DeltaDims& d, int64_t* st, int64_t* ut, int64_t* wt, int64_t* gc, int64_t* end) {
-  *st = 0;
-  *ut = *st + d.chunks * d.Vp * d.Kp;
-  *wt = *ut + d.chunks * d.Vp * kC;
-  *gc = *wt + d.chunks * d.Kp * kC;
-  *end = *gc + ((d.chunks + 3) & ~(int64_t)3);
-}
-
-extern "C" int64_t ope_delta_saved_bytes(const ope_delta_cfg* cfg) {
-  if (!delta_ok(cfg)) return OPE_EINVAL;
-  int64_t a, b, c, e, end;
-  saved_layout(delta_dims(cfg), &a, &b, &c, &e, &end);
-  return end * 4;
-}
-
 namespace ope {
-void delta_saved(const DeltaDims& d, float* saved, float** ST, float** UT, float** WT, float** gC) {
-  int64_t a, b, c, e, end;
-  saved_layout(d, &a, &b, &c, &e, &end);
-  *ST = saved + a; *UT = saved + b; *WT = saved + c; *gC = saved + e;
+// the arrays of `saved`, in the order the header of ope_delta.h names them; returns its floats
+int64_t delta_saved(const DeltaDims& d, float* saved, float** ST, float** UT, float** WT, float** gC, float** tails) {
+  const int64_t ut = d.chunks * d.Vp * d.Kp, wt = ut + d.chunks * d.Vp * kC, tl = wt + d.chunks * d.Kp * kC, gc = tl + d.chunks * kC;
+  *ST = saved; *UT = saved + ut; *WT = saved + wt; *tails = saved + tl; *gC = saved + gc;
+  return gc + ((d.chunks + 3) & ~(int64_t)3);
 }
 int64_t delta_bwd_floats(const DeltaDims& d) {
   return d.chunks * ((int64_t)kC * d.Kp + (int64_t)d.Vp * kC + (int64_t)d.Vp * d.Kp) + (d.H != d.Hk ? 2 * (int64_t)d.B * d.T * d.H * d.K : 0);
 }
+}
+
+extern "C" int64_t ope_delta_saved_bytes(const ope_delta_cfg* cfg) {
+  if (!delta_ok(cfg)) return OPE_EINVAL;
+  float *a, *b, *c, *e, *f;
+  return 4 * delta_saved(delta_dims(cfg), nullptr, &a, &b, &c, &e, &f);
 }
 
 extern "C" int64_t ope_delta_workspace_bytes(const ope_delta_cfg* cfg, int32_t backward) {
@@ -365,18 +411,19 @@ extern "C" int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const 
   }
   if (!q || !k || !v || !g || !beta || !o || !saved || !workspace) return OPE_EINVAL;
   if (saved_bytes < ope_delta_saved_bytes(cfg) || workspace_bytes < ope_delta_workspace_bytes(cfg, 0)) return OPE_ENOSPC;
-  float *ST, *UT, *WT, *gC;
-  delta_saved(d, (float*)saved, &ST, &UT, &WT, &gC);
-  float *W = (float*)workspace, *KdT = W + d.chunks * kC * d.Kp;
+  float *ST, *UT, *WT, *gC, *tails;
+  delta_saved(d, (float*)saved, &ST, &UT, &WT, &gC, &tails);
+  float* W = (float*)workspace;
+  void* KTs = W + d.chunks * kC * d.Kp;
   return with_elem(cfg->dtype, [&](auto t) {
     typedef decltype(t) T;
     const dim3 grid((unsigned)d.chunks);
 #define OPE_PREP(KT) \
-  case KT: OPE_LAUNCH((delta_prep<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)k, (const T*)v, g, beta, lengths, W, WT, KdT, UT, gC); break
+  case KT: OPE_LAUNCH((delta_prep<T, KT>), grid, dim3(64 * chunk_waves<KT>()), 0, st, *cfg, d, (const T*)k, (const T*)v, g, beta, lengths, W, WT, (T*)KTs, UT, gC, tails); break
     switch (d.KT) { OPE_PREP(1); OPE_PREP(2); OPE_PREP(4); OPE_PREP(8); }
 #undef OPE_PREP
     OPE_CHECK_LAUNCH();
-    const int rc = launch_delta_scan(d, false, lengths, W, KdT, UT, ST, gC, state0, state_out, st);
+    const int rc = launch_delta_scan(cfg->dtype, d, false, lengths, W, KTs, UT, ST, gC, tails, state0, state_out, st);
     if (rc) return rc;
 #define OPE_OUT(KT) \
   case KT: OPE_LAUNCH((delta_out<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, ST, UT, (T*)o); break

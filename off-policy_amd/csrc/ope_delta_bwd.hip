@@ -16,35 +16,37 @@
 
 namespace ope {
 
-int launch_delta_scan(const DeltaDims& d, bool bwd, const int32_t* lengths, const float* M1, const float* M2, float* UT, float* ST, const float* gC,
-                      const float* first, float* last, hipStream_t st);
-void delta_saved(const DeltaDims& d, float* saved, float** ST, float** UT, float** WT, float** gC);
+int launch_delta_scan(int dtype, const DeltaDims& d, bool bwd, const int32_t* lengths, const void* M1, const void* M2, float* UT, float* ST,
+                      const float* gC, const float* tails, const float* first, float* last, hipStream_t st);
+int64_t delta_saved(const DeltaDims& d, float* saved, float** ST, float** UT, float** WT, float** gC, float** tails);
 __global__ void delta_keep_state(const float* __restrict__ from, float* __restrict__ to, int64_t n);
 
 template <typename T, int KT>
-__global__ __launch_bounds__(256) void delta_bwd_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
-                                                      const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
-                                                      const T* __restrict__ dO, float* __restrict__ Kd, float* __restrict__ dUT, float* __restrict__ dST) {
-  constexpr int Kp = 16 * KT;
-  __shared__ float q[kC][Kp + 4], k[kC][Kp + 4], PT[kC][kC + 4];
+__global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta_bwd_prep(
+    ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in, const float* __restrict__ g_in, const float* __restrict__ beta_in,
+    const int32_t* __restrict__ lengths, const T* __restrict__ dO, T* __restrict__ Ks, float* __restrict__ dUT, float* __restrict__ dST) {
+  constexpr int NW = chunk_waves<KT>(), RS = Rows<T, KT>::kStride;
+  __shared__ Rows<T, KT> q, k;
+  __shared__ float PT[kC][kC + 4];
   __shared__ Gates gt;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
   if (a.nv == 0) return;
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
   const int hk = a.h / (d.H / d.Hk);
-  load_rows<T, KT>(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows<T, KT>(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
-  for (int x = threadIdx.x; x < kC * KT * 4; x += 256) {
-    const int t = x / (KT * 4), f = (x % (KT * 4)) * 4;
-    put4(&Kd[(a.c * kC + t) * Kp + f], at4(&k[t][f]) * gt.tail[t]);
-  }
-  const int s = 16 * w + j;
-  for (int it = w; it < 4; ++it) {
+  for (int x = w; x < 4 * KT; x += NW)                   // k, a tile a wave
+    *reinterpret_cast<typename Pack<T, 4>::vec*>(Ks + (a.c * 4 * KT + x) * 256 + tile_lane()) =
+        *reinterpret_cast<const typename Pack<T, 4>::vec*>(&k.v[16 * (x / KT) + j][16 * (x % KT) + 4 * g]);
+  for (int x = w; x < 10; x += NW) {
+    int it, is;
+    lower_tile(x, it, is);
+    const int s = 16 * is + j;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < KT; ++c) acc = mfma4(at4(&q[16 * it + j][16 * c + 4 * g]), at4(&k[s][16 * c + 4 * g]), acc);
+    for (int c = 0; c < KT; ++c) acc = dot4(&q.v[16 * it + j][16 * c + 4 * g], &k.v[s][16 * c + 4 * g], acc);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * it + 4 * g + r;
@@ -54,46 +56,51 @@ __global__ __launch_bounds__(256) void delta_bwd_prep(ope_delta_cfg cfg, DeltaDi
   }
   __syncthreads();
   const T* o0 = dO + a.b * cfg.o_stride[0] + (int64_t)a.t0 * cfg.o_stride[1] + a.h * cfg.o_stride[2];
-  for (int vt = w; vt < d.VT; vt += 4) {
+  for (int vt = w; vt < d.VT; vt += NW) {
     const int v = 16 * vt + j;
-    f32x4 x[4], y[4];
+    f32x4 x[4];
 #pragma unroll
     for (int it = 0; it < 4; ++it)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int t = 16 * it + 4 * g + r;
         x[it][r] = t < a.nv && v < d.V ? (float)o0[(int64_t)t * cfg.o_stride[1] + v] : 0.f;
-        y[it][r] = x[it][r] * cfg.scale * gt.head[t];
       }
 #pragma unroll
     for (int is = 0; is < 4; ++is) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int it = is; it < 4; ++it) acc = mfma4(at4(&PT[16 * is + j][16 * it + 4 * g]), x[it], acc);
-      put4(&dUT[(a.c * d.Vp + v) * kC + 16 * is + 4 * g], acc);
+      put4(&dUT[((a.c * d.VT + vt) * 4 + is) * 256 + tile_lane()], acc);
     }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.head[16 * it + 4 * g]) * cfg.scale;
+#pragma unroll 2
     for (int kt = 0; kt < KT; ++kt) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int it = 0; it < 4; ++it) acc = mfma4(col4(&q[16 * it + 4 * g][16 * kt + j], Kp + 4), y[it], acc);
-      put4(&dST[(a.c * d.Vp + v) * Kp + 16 * kt + 4 * g], acc);
+      for (int it = 0; it < 4; ++it) acc = mfma4(column4(&q.v[16 * it + 4 * g][16 * kt + j], RS), x[it], acc);
+      put4(&dST[((a.c * d.VT + vt) * KT + kt) * 256 + tile_lane()], acc);
     }
   }
 }
 
-// Wave w owns the tokens 16w.. as data rows; the three products over the value columns keep 3 * KT accumulators in registers, so S, dS' and U
-// are read once a wave. One workgroup a CU at Kp = 128 (130 KB of LDS).
+// Eight waves: wave w owns the tokens 16 (w & 3).. as data rows and one half (w >> 2) of the key tiles, so the three products over the value
+// columns keep 3 * KT / 2 accumulators in registers and S, dS' are read by four waves instead of eight. The first half makes dP, the second
+// dA; they change hands through LDS, where dP takes the place of A once the triangular solve is done.
 template <typename T, int KT>
-__global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
+__global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_main(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
                                                       const T* __restrict__ v_in, const float* __restrict__ g_in, const float* __restrict__ beta_in,
                                                       const int32_t* __restrict__ lengths, const float* __restrict__ ST, const float* __restrict__ UT,
                                                       const T* __restrict__ dO, float* dUT, const float* __restrict__ dST, T* __restrict__ dq,
                                                       T* __restrict__ dk, float* __restrict__ dqp, float* __restrict__ dkp, T* __restrict__ dv,
                                                       float* __restrict__ dg, float* __restrict__ dbeta) {
-  constexpr int Kp = 16 * KT;
-  __shared__ float q[kC][Kp + 4], k[kC][Kp + 4], NA[kC][kC + 4], inv[4][16][20], dPs[kC][kC + 4], dAs[kC][kC + 4];
-  __shared__ float dbv[4][kC], dG[kC], dEnd[kC], dots[4];
+  constexpr int RS = Rows<T, KT>::kStride, KH = (KT + 1) / 2;      // KH: key tiles of a half
+  __shared__ Rows<T, KT> q, k;
+  __shared__ float NA[kC][kC + 4], dAs[kC][kC + 4], inv[4][16][20];
+  __shared__ float dbv[8][kC], sums[2][4][kC], dots[8];
   __shared__ Gates gt;
+  float(*dPs)[kC + 4] = NA;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   const int rows = min(d.T - a.t0, kC), hk = a.h / (d.H / d.Hk);
@@ -121,8 +128,8 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
     }
   };
   if (a.nv == 0) {
-    for (int x = threadIdx.x; x < rows * d.V; x += 256) dv0[(int64_t)(x / d.V) * cfg.dv_stride[1] + x % d.V] = (T)0.f;
-    for (int x = threadIdx.x; x < kC * KT * 4; x += 256) {
+    for (int x = threadIdx.x; x < rows * d.V; x += 512) dv0[(int64_t)(x / d.V) * cfg.dv_stride[1] + x % d.V] = (T)0.f;
+    for (int x = threadIdx.x; x < kC * KT * 4; x += 512) {
       const int t = x / (KT * 4), f = (x % (KT * 4)) * 4;
       put_k(dq, cfg.dq_stride, dqp, t, f, f32x4{0.f, 0.f, 0.f, 0.f});
       put_k(dk, cfg.dk_stride, dkp, t, f, f32x4{0.f, 0.f, 0.f, 0.f});
@@ -134,10 +141,10 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
     return;
   }
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
-  load_rows<T, KT>(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows<T, KT>(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
-  minus_A<KT>(NA, k, gt);
+  minus_A<T, KT>(NA, k, gt);
   __syncthreads();
   if (w == 0) diag_inverse(inv, NA);
   __syncthreads();
@@ -147,18 +154,18 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
     f32x4 part[4];
 #pragma unroll
     for (int it = 0; it < 4; ++it) part[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int vt = w; vt < d.VT; vt += 4) {
+    for (int vt = w; vt < d.VT; vt += 8) {
       const int v = 16 * vt + j;
       f32x4 x[4];
 #pragma unroll
-      for (int it = 0; it < 4; ++it) x[it] = at4(&dUT[(a.c * d.Vp + v) * kC + 16 * it + 4 * g]);
+      for (int it = 0; it < 4; ++it) x[it] = at4(&dUT[((a.c * d.VT + vt) * 4 + it) * 256 + tile_lane()]);
 #pragma unroll
       for (int it = 3; it >= 0; --it) {
         f32x4 acc = x[it];
 #pragma unroll
         for (int kt = it + 1; kt < 4; ++kt) acc = mfma4(col4(&NA[16 * kt + 4 * g][16 * it + j], kC + 4), x[kt], acc);
         x[it] = mfma4(col4(&inv[it][4 * g][j], 20), acc, f32x4{0.f, 0.f, 0.f, 0.f});
-        put4(&dUT[(a.c * d.Vp + v) * kC + 16 * it + 4 * g], x[it]);
+        put4(&dUT[((a.c * d.VT + vt) * 4 + it) * 256 + tile_lane()], x[it]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = 16 * it + 4 * g + r;
@@ -175,13 +182,13 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
         if (j == 0) dbv[w][16 * it + 4 * g + r] = x;
       }
   }
-  __syncthreads();     // dR of all columns is in dUT
-  const int t = 16 * w + j;
-  f32x4 X1[KT], X2[KT], X3[KT], P[4], A[4];
+  __syncthreads();     // dR of all columns is in dUT; A is done with
+  const int wt = w & 3, half = w >> 2, k0 = half * KH, t = 16 * wt + j;
+  f32x4 X1[KH], X2[KH], X3[KH], M[4];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) X1[kt] = X2[kt] = X3[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int q = 0; q < KH; ++q) X1[q] = X2[q] = X3[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int is = 0; is < 4; ++is) P[is] = A[is] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int is = 0; is < 4; ++is) M[is] = f32x4{0.f, 0.f, 0.f, 0.f};
   float dot = 0.f;
   const T* o0 = dO + a.b * cfg.o_stride[0] + (int64_t)(a.t0 + t) * cfg.o_stride[1] + a.h * cfg.o_stride[2];
   for (int vt = 0; vt < d.VT; ++vt) {
@@ -194,25 +201,24 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
         for (int e = 0; e < 4; ++e)
           if (v + e < d.V) bo[e] = (float)o0[v + e];
     }
-    const float* S0 = ST + (a.c * d.Vp + v) * Kp + j;
-    const float* D0 = dST + (a.c * d.Vp + v) * Kp + j;
-    const float* U0 = UT + (a.c * d.Vp + v) * kC + j;
-    const f32x4 br = col4(dUT + (a.c * d.Vp + v) * kC + t, kC), bu = col4(U0 + 16 * w, kC);
+    const int64_t at = a.c * d.VT + vt;
+    const float* S0 = ST + at * KT * 256 + turned_lane();
+    const float* D0 = dST + at * KT * 256 + turned_lane();
+    const float* U0 = UT + at * 4 * 256 + turned_lane();
+    const f32x4 br = turn4(at4(dUT + (at * 4 + wt) * 256 + turned_lane())), bu = turn4(at4(U0 + wt * 256));
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const f32x4 s = col4(S0 + 16 * kt, Kp), ds = col4(D0 + 16 * kt, Kp);
-      X1[kt] = mfma4(s, bo, X1[kt]);
-      X2[kt] = mfma4(s, br, X2[kt]);
-      X3[kt] = mfma4(ds, bu, X3[kt]);
-      if ((kt & 3) == w) dot += s[0] * ds[0] + s[1] * ds[1] + s[2] * ds[2] + s[3] * ds[3];
-    }
+    for (int q = 0; q < KH; ++q)
+      if (k0 + q < KT) {
+        const f32x4 s = turn4(at4(S0 + (k0 + q) * 256)), ds = turn4(at4(D0 + (k0 + q) * 256));
+        X1[q] = mfma4(s, bo, X1[q]);
+        X2[q] = mfma4(s, br, X2[q]);
+        X3[q] = mfma4(ds, bu, X3[q]);
+        if ((q & 3) == wt) dot += s[0] * ds[0] + s[1] * ds[1] + s[2] * ds[2] + s[3] * ds[3];
+      }
+    const f32x4 bm = half ? br : bo;
 #pragma unroll
     for (int is = 0; is < 4; ++is)
-      if (is <= w) {
-        const f32x4 u = col4(U0 + 16 * is, kC);
-        P[is] = mfma4(u, bo, P[is]);
-        A[is] = mfma4(u, br, A[is]);
-      }
+      if (is <= wt) M[is] = mfma4(turn4(at4(U0 + is * 256)), bm, M[is]);
   }
   dot = rowsum4(row16_sum(dot));
   if ((threadIdx.x & 63) == 0) dots[w] = dot;
@@ -222,64 +228,80 @@ __global__ __launch_bounds__(256) void delta_bwd_main(ope_delta_cfg cfg, DeltaDi
     for (int r = 0; r < 4; ++r) {
       const int s = 16 * is + 4 * g + r;
       const float dec = s <= t ? decay(gt, t, s) : 0.f;
-      P[is][r] = P[is][r] * cfg.scale * dec;
-      A[is][r] = s < t ? -A[is][r] * dec : 0.f;
+      M[is][r] = half ? (s < t ? -M[is][r] * dec : 0.f) : M[is][r] * cfg.scale * dec;
     }
-    put4(&dPs[t][16 * is + 4 * g], P[is]);
-    put4(&dAs[t][16 * is + 4 * g], A[is] * gt.beta[t]);
-  }
-  const float fq = cfg.scale * gt.head[t], fr = gt.head[t];
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    X1[kt] *= fq;
-    X2[kt] *= -fr;
-#pragma unroll
-    for (int is = 0; is < 4; ++is)
-      if (is <= w) {
-        const f32x4 kc = col4(&k[16 * is + 4 * g][16 * kt + j], Kp + 4);
-        X1[kt] = mfma4(kc, P[is], X1[kt]);        // dq
-        X2[kt] = mfma4(kc, A[is], X2[kt]);        // the terms of dk that carry beta_t, without it
-      }
+    put4(half ? &dAs[t][16 * is + 4 * g] : &dPs[t][16 * is + 4 * g], M[is]);      // dP scale decay, dA decay (without beta_t)
   }
   __syncthreads();
-  float pq = 0.f, pr = 0.f, pc = 0.f, ps = 0.f;
-  const float bt = gt.beta[t], tail = gt.tail[t];
+  const float fq = cfg.scale * gt.head[t], fr = gt.head[t], bt = gt.beta[t], tail = gt.tail[t];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    f32x4 c = {0.f, 0.f, 0.f, 0.f};
-    for (int it = w; it < 4; ++it) {
-      c = mfma4(col4(&q[16 * it + 4 * g][16 * kt + j], Kp + 4), col4(&dPs[16 * it + 4 * g][t], kC + 4), c);
-      c = mfma4(col4(&k[16 * it + 4 * g][16 * kt + j], Kp + 4), col4(&dAs[16 * it + 4 * g][t], kC + 4), c);
-    }
-    const int f = 16 * kt + 4 * g;
-    const f32x4 kv = at4(&k[t][f]), qv = at4(&q[t][f]), e = X3[kt] * tail;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      pq = fmaf(qv[r], X1[kt][r], pq);
-      pr = fmaf(kv[r], X2[kt][r], pr);
-      pc = fmaf(kv[r], c[r], pc);
-      ps = fmaf(kv[r], e[r], ps);
-    }
-    put_k(dq, cfg.dq_stride, dqp, t, f, X1[kt]);
-    put_k(dk, cfg.dk_stride, dkp, t, f, X2[kt] * bt + c + e);
+  for (int q = 0; q < KH; ++q) {
+    X1[q] *= fq;
+    X2[q] *= -fr;
   }
+  for (int is = 0; is <= wt; ++is) {
+    const f32x4 bp = at4(&dPs[t][16 * is + 4 * g]), ba = at4(&dAs[t][16 * is + 4 * g]);
+#pragma unroll
+    for (int q = 0; q < KH; ++q)
+      if (k0 + q < KT) {
+        const f32x4 kc = column4(&k.v[16 * is + 4 * g][16 * (k0 + q) + j], RS);
+        X1[q] = mfma4(kc, bp, X1[q]);              // dq
+        X2[q] = mfma4(kc, ba, X2[q]);              // the terms of dk that carry beta_t, without it
+      }
+  }
+  f32x4 C[KH];
+#pragma unroll
+  for (int q = 0; q < KH; ++q) C[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int it = wt; it < 4; ++it) {
+    const f32x4 bp = col4(&dPs[16 * it + 4 * g][t], kC + 4), ba = col4(&dAs[16 * it + 4 * g][t], kC + 4) * at4(&gt.beta[16 * it + 4 * g]);
+#pragma unroll
+    for (int i = 0; i < KH; ++i)
+      if (k0 + i < KT) {
+        C[i] = mfma4(column4(&q.v[16 * it + 4 * g][16 * (k0 + i) + j], RS), bp, C[i]);
+        C[i] = mfma4(column4(&k.v[16 * it + 4 * g][16 * (k0 + i) + j], RS), ba, C[i]);
+      }
+  }
+  float pq = 0.f, pr = 0.f, pc = 0.f, ps = 0.f;
+#pragma unroll
+  for (int i = 0; i < KH; ++i)
+    if (k0 + i < KT) {
+      const int f = 16 * (k0 + i) + 4 * g;
+      const f32x4 kv = row4(&k.v[t][f]), qv = row4(&q.v[t][f]), e = X3[i] * tail;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        pq = fmaf(qv[r], X1[i][r], pq);
+        pr = fmaf(kv[r], X2[i][r], pr);
+        pc = fmaf(kv[r], C[i][r], pc);
+        ps = fmaf(kv[r], e[r], ps);
+      }
+      put_k(dq, cfg.dq_stride, dqp, t, f, X1[i]);
+      put_k(dk, cfg.dk_stride, dkp, t, f, X2[i] * bt + C[i] + e);
+    }
   pq = rowsum4(pq); pr = rowsum4(pr); pc = rowsum4(pc); ps = rowsum4(ps);
   if (g == 0) {
-    dG[t] = pq + bt * pr - pc - ps;
-    dEnd[t] = ps;
-    if (t < rows) db0[(int64_t)t * cfg.dbeta_stride[1]] = t < a.nv ? pr + dbv[0][t] + dbv[1][t] + dbv[2][t] + dbv[3][t] : 0.f;
+    sums[half][0][t] = pq;
+    sums[half][1][t] = pr;
+    sums[half][2][t] = pc;
+    sums[half][3][t] = ps;
   }
   __syncthreads();
   if (w == 0) {
     const int l = threadIdx.x, seg = gt.seg[l];
-    double x = dG[l], end = dEnd[l];
+    const float r = sums[0][1][l] + sums[1][1][l];
+    float db = r;
+    for (int i = 0; i < 8; ++i) db += dbv[i][l];
+    if (l < rows) db0[(int64_t)l * cfg.dbeta_stride[1]] = l < a.nv ? db : 0.f;
+    double end = (double)sums[0][3][l] + sums[1][3][l];
+    double x = (double)sums[0][0][l] + sums[1][0][l] + gt.beta[l] * (double)r - sums[0][2][l] - sums[1][2][l] - end;
     for (int m = 1; m < 64; m <<= 1) {
       const double o = __shfl_down(x, m, 64);
       const int so = __shfl_down(seg, m, 64);
       if (l + m < 64 && so == seg) x += o;
       end += __shfl_xor(end, m, 64);
     }
-    end += (double)gt.whole * ((double)dots[0] + dots[1] + dots[2] + dots[3]);
+    double dot_all = 0.0;
+    for (int i = 0; i < 8; ++i) dot_all += dots[i];
+    end += (double)gt.whole * dot_all;
     if (seg == gt.seg[63]) x += end;
     const bool cut = seg != (l > 0 ? gt.seg[l - 1] : 0);       // g = -inf here
     if (l < rows) dg0[(int64_t)l * cfg.dg_stride[1]] = l < a.nv && !cut ? (float)x : 0.f;
@@ -322,10 +344,10 @@ extern "C" int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const
   }
   if (!q || !k || !v || !g || !beta || !saved || !d_o || !dq || !dk || !dv || !dg || !dbeta || !workspace) return OPE_EINVAL;
   if (saved_bytes < ope_delta_saved_bytes(cfg) || workspace_bytes < ope_delta_workspace_bytes(cfg, 1)) return OPE_ENOSPC;
-  float *ST, *UT, *WT, *gC;
-  delta_saved(d, (float*)saved, &ST, &UT, &WT, &gC);
-  float* Kd = (float*)workspace;
-  float* dUT = Kd + d.chunks * kC * d.Kp;
+  float *ST, *UT, *WT, *gC, *tails;
+  delta_saved(d, (float*)saved, &ST, &UT, &WT, &gC, &tails);
+  void* Ks = workspace;
+  float* dUT = (float*)workspace + d.chunks * kC * d.Kp;
   float* dST = dUT + d.chunks * d.Vp * kC;
   float* dqp = dST + d.chunks * d.Vp * d.Kp;
   float* dkp = dqp + (int64_t)d.B * d.T * d.H * d.K;
@@ -333,14 +355,14 @@ extern "C" int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const
     typedef decltype(t) T;
     const dim3 grid((unsigned)d.chunks);
 #define OPE_BPREP(KT) \
-  case KT: OPE_LAUNCH((delta_bwd_prep<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, (const T*)d_o, Kd, dUT, dST); break
+  case KT: OPE_LAUNCH((delta_bwd_prep<T, KT>), grid, dim3(64 * chunk_waves<KT>()), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, (const T*)d_o, (T*)Ks, dUT, dST); break
     switch (d.KT) { OPE_BPREP(1); OPE_BPREP(2); OPE_BPREP(4); OPE_BPREP(8); }
 #undef OPE_BPREP
     OPE_CHECK_LAUNCH();
-    const int rc = launch_delta_scan(d, true, lengths, Kd, WT, dUT, dST, gC, d_state, d_state0, st);
+    const int rc = launch_delta_scan(cfg->dtype, d, true, lengths, Ks, WT, dUT, dST, gC, tails, d_state, d_state0, st);
     if (rc) return rc;
 #define OPE_BMAIN(KT)                                                                                                                                  \
-  case KT: OPE_LAUNCH((delta_bwd_main<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)q, (const T*)k, (const T*)v, g, beta, lengths, ST, UT,        \
+  case KT: OPE_LAUNCH((delta_bwd_main<T, KT>), grid, dim3(512), 0, st, *cfg, d, (const T*)q, (const T*)k, (const T*)v, g, beta, lengths, ST, UT,        \
                       (const T*)d_o, dUT, dST, (T*)dq, (T*)dk, dqp, dkp, (T*)dv, dg, dbeta); break
     switch (d.KT) { OPE_BMAIN(1); OPE_BMAIN(2); OPE_BMAIN(4); OPE_BMAIN(8); }
 #undef OPE_BMAIN
