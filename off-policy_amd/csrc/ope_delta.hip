@@ -120,23 +120,24 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
       const int k = 16 * (w + 4 * q) + 4 * g + r;
       S[q][r] = first && k < d.K && v < d.V ? first[(bh * d.K + k) * d.V + v] : 0.f;
     }
-  auto fetch = [&](Ops& o, int s) {       // step s of the walk; past the end: the last one again
-    const int64_t c = bh * d.n + (BWD ? n - 1 - min(s, n - 1) : min(s, n - 1));
-#pragma unroll
-    for (int q = 0; q < KT; ++q) o.m1[q] = *reinterpret_cast<const decltype(o.m1[0] + o.m1[0])*>(M1 + ((c * 4 + w) * KT + q) * 256 + lane);
+  typedef decltype(Ops().m1[0] + Ops().m1[0]) V1;
+  typedef decltype(Ops().m2[0][0] + Ops().m2[0][0]) V2;
+  auto at = [&](int s) { return bh * d.n + (BWD ? n - 1 - min(s, n - 1) : min(s, n - 1)); };     // chunk of step s; past the end: the last one again
+  auto get1 = [&](Ops& o, int64_t c, int q) { o.m1[q] = *reinterpret_cast<const V1*>(M1 + ((c * 4 + w) * KT + q) * 256 + lane); };
+  auto get2 = [&](Ops& o, int64_t c, int q, int p) { o.m2[q][p] = *reinterpret_cast<const V2*>(M2 + ((c * KT + min(w + 4 * q, KT - 1)) * 4 + p) * 256 + lane); };
+  auto get_rest = [&](Ops& o, int64_t c) {
     o.u = at4(&UT[((c * VT + vt) * 4 + w) * 256 + lane]);
+    if (BWD)
 #pragma unroll
-    for (int q = 0; q < NK; ++q) {
-      const int kt = min(w + 4 * q, KT - 1);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) o.m2[q][p] = *reinterpret_cast<const decltype(o.m2[0][0] + o.m2[0][0])*>(M2 + ((c * KT + kt) * 4 + p) * 256 + lane);
-      if (BWD) o.add[q] = at4(&ST[((c * VT + vt) * KT + kt) * 256 + lane]);
-    }
+      for (int q = 0; q < NK; ++q) o.add[q] = at4(&ST[((c * VT + vt) * KT + min(w + 4 * q, KT - 1)) * 256 + lane]);
     o.tail = at4(&tails[c * kC + 16 * w + 4 * g]);
     o.whole = gC[c];
   };
+  // The operands of the step after next are loaded one by one, each behind the product that read its registers last: in one burst they hold up
+  // the wave until the CU has taken them all (measured: 2.4 us a chunk at Kp = 128, 1.3 without any loads), and left to itself the compiler moves
+  // them to the front, into registers of their own, and waits for the copies. (M1, M2 are not __restrict__ for the same reason.)
   auto step = [&](Ops& o, int s) {
-    const int64_t c = bh * d.n + (BWD ? n - 1 - s : s);
+    const int64_t c = at(s), next = at(s + 2);
 #pragma unroll
     for (int q = 0; q < NK; ++q)
       if (KT % 4 == 0 || w + 4 * q < KT) {
@@ -144,32 +145,49 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
         put4(&ST[((c * VT + vt) * KT + w + 4 * q) * 256 + lane], S[q]);
       }
     lds_barrier();
-    f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
+    f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0, x[KT > 4 ? KT : 4];
+#pragma unroll
+    for (int q = 0; q < KT; ++q) x[q] = at4(&SL[j][16 * q + 4 * g]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < KT; ++q) {
       f32x4& p = q & 1 ? p1 : p0;
-      p = mfma4(__builtin_convertvector(o.m1[q], f32x4), at4(&SL[j][16 * q + 4 * g]), p);
+      p = mfma4(__builtin_convertvector(o.m1[q], f32x4), x[q], p);
+      get1(o, next, q);
+      __builtin_amdgcn_sched_barrier(0);
     }
     const f32x4 u = BWD ? o.u + o.tail * (p0 + p1) : o.u - (p0 + p1);
     put4(&UL[j][16 * w + 4 * g], BWD ? u : u * o.tail);
     put4(&UT[((c * VT + vt) * 4 + w) * 256 + lane], u);
     lds_barrier();
 #pragma unroll
+    for (int p = 0; p < 4; ++p) x[p] = at4(&UL[j][16 * p + 4 * g]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
     for (int q = 0; q < NK; ++q)
       if (KT % 4 == 0 || w + 4 * q < KT) {
         f32x4 a0 = {0.f, 0.f, 0.f, 0.f}, a1 = a0;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          f32x4& x = p & 1 ? a1 : a0;
-          x = mfma4(__builtin_convertvector(o.m2[q][p], f32x4), at4(&UL[j][16 * p + 4 * g]), x);
+          f32x4& acc = p & 1 ? a1 : a0;
+          acc = mfma4(__builtin_convertvector(o.m2[q][p], f32x4), x[p], acc);
+          get2(o, next, q, p);
+          __builtin_amdgcn_sched_barrier(0);
         }
         S[q] = BWD ? o.whole * S[q] + o.add[q] - (a0 + a1) : o.whole * S[q] + (a0 + a1);
       }
-    // Here and no earlier: hoisted above the products (the compiler's own wish) these loads need registers of their own, and the copies into the
-    // loop's wait for them at once. (M1, M2 are not __restrict__ for the same reason.)
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-    fetch(o, s + 2);
+    get_rest(o, next);
+  };
+  auto fetch = [&](Ops& o, int s) {
+    const int64_t c = at(s);
+#pragma unroll
+    for (int q = 0; q < KT; ++q) get1(o, c, q);
+#pragma unroll
+    for (int q = 0; q < NK; ++q)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) get2(o, c, q, p);
+    get_rest(o, c);
   };
   if (n > 0) {
     Ops even, odd;
