@@ -13,7 +13,7 @@
 //   WT  [c][KT][4]   float32 S  W transposed: rows k, columns t
 //   gC  [c]          float32 S  decay over the whole chunk (0 behind a reset);  tails [c][64] float32 S  decay from t to the chunk's end
 //   W   [c][4][KT]   float32 W  rows t, columns k                                KTs [c][KT][4] of the inputs' type W  k transposed: rows k, columns t
-//   backward: Ks [c][4][KT] of the inputs' type W (rows t, columns k), dUT like UT (dU0, then dU, then dR), dST like ST (N, then the gradient of the
+//   backward: Ks [c][4][KT] of the inputs' type W (rows t, columns k), dUT like UT (dU0, then dU, then dR with its tiles transposed), dST like ST (N, then the gradient of the
 //   state BEHIND the chunk), dqp, dkp [b][t][H][K] float32 where query / key heads are shared
 #pragma once
 #include <type_traits>

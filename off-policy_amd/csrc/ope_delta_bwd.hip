@@ -98,7 +98,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   constexpr int RS = Rows<T, KT>::kStride, KH = (KT + 1) / 2;      // KH: key tiles of a half
   __shared__ Rows<T, KT> q, k;
   __shared__ float NA[kC][kC + 4], dAs[kC][kC + 4], inv[4][16][20];
-  __shared__ float dbv[8][kC], sums[2][4][kC], dots[8];
+  __shared__ float dbv[2][kC], sums[2][4][kC], dots[8];
   __shared__ Gates gt;
   float(*dPs)[kC + 4] = NA;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
@@ -148,39 +148,20 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   __syncthreads();
   if (w == 0) diag_inverse(inv, NA);
   __syncthreads();
-  // dR = (I + A)^-T dU, block backward substitution, 16 value columns a wave at a time; dv; the part of dbeta that v gives
-  {
-    const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)a.t0 * cfg.v_stride[1] + a.h * cfg.v_stride[2];
-    f32x4 part[4];
+  // dR = (I + A)^-T dU, block backward substitution, 16 value columns a wave at a time; left in dUT with its tiles transposed
+  for (int vt = w; vt < d.VT; vt += 8) {
+    float* at = dUT + (a.c * d.VT + vt) * 4 * 256;
+    f32x4 x[4];
 #pragma unroll
-    for (int it = 0; it < 4; ++it) part[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int vt = w; vt < d.VT; vt += 8) {
-      const int v = 16 * vt + j;
-      f32x4 x[4];
+    for (int it = 0; it < 4; ++it) x[it] = at4(at + it * 256 + tile_lane());
 #pragma unroll
-      for (int it = 0; it < 4; ++it) x[it] = at4(&dUT[((a.c * d.VT + vt) * 4 + it) * 256 + tile_lane()]);
+    for (int it = 3; it >= 0; --it) {
+      f32x4 acc = x[it];
 #pragma unroll
-      for (int it = 3; it >= 0; --it) {
-        f32x4 acc = x[it];
-#pragma unroll
-        for (int kt = it + 1; kt < 4; ++kt) acc = mfma4(col4(&NA[16 * kt + 4 * g][16 * it + j], kC + 4), x[kt], acc);
-        x[it] = mfma4(col4(&inv[it][4 * g][j], 20), acc, f32x4{0.f, 0.f, 0.f, 0.f});
-        put4(&dUT[((a.c * d.VT + vt) * 4 + it) * 256 + tile_lane()], x[it]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = 16 * it + 4 * g + r;
-          if (t < rows && v < d.V) dv0[(int64_t)t * cfg.dv_stride[1] + v] = (T)(t < a.nv ? gt.beta[t] * x[it][r] : 0.f);
-          if (t < a.nv && v < d.V) part[it][r] = fmaf(x[it][r], (float)v0[(int64_t)t * cfg.v_stride[1] + v], part[it][r]);
-        }
-      }
+      for (int kt = it + 1; kt < 4; ++kt) acc = mfma4(col4(&NA[16 * kt + 4 * g][16 * it + j], kC + 4), x[kt], acc);
+      x[it] = mfma4(col4(&inv[it][4 * g][j], 20), acc, f32x4{0.f, 0.f, 0.f, 0.f});
+      put4(at + it * 256 + turned_lane(), turn4(x[it]));
     }
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = row16_sum(part[it][r]);
-        if (j == 0) dbv[w][16 * it + 4 * g + r] = x;
-      }
   }
   __syncthreads();     // dR of all columns is in dUT; A is done with
   const int wt = w & 3, half = w >> 2, k0 = half * KH, t = 16 * wt + j;
@@ -189,23 +170,29 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   for (int q = 0; q < KH; ++q) X1[q] = X2[q] = X3[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int is = 0; is < 4; ++is) M[is] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float dot = 0.f;
+  float dot = 0.f, rv = 0.f;                          // <dS', S> and dR.v of the tiles this wave counts
   const T* o0 = dO + a.b * cfg.o_stride[0] + (int64_t)(a.t0 + t) * cfg.o_stride[1] + a.h * cfg.o_stride[2];
-  for (int vt = 0; vt < d.VT; ++vt) {
-    const int v = 16 * vt + 4 * g;
-    f32x4 bo = {0.f, 0.f, 0.f, 0.f};
+  const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)(a.t0 + t) * cfg.v_stride[1] + a.h * cfg.v_stride[2];
+  // four values of a row from column v on; nothing is read past the row's end or behind the last live token
+  auto value4 = [&](const T* row, int v) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
     if (t < a.nv) {
-      if (v + 4 <= d.V) bo = load_pack<T, 4>(o0 + v);
+      if (v + 4 <= d.V) x = load_pack<T, 4>(row + v);
       else
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (v + e < d.V) bo[e] = (float)o0[v + e];
+          if (v + e < d.V) x[e] = (float)row[v + e];
     }
+    return x;
+  };
+  for (int vt = 0; vt < d.VT; ++vt) {
+    const int v = 16 * vt + 4 * g;
+    const f32x4 bo = value4(o0, v);
     const int64_t at = a.c * d.VT + vt;
     const float* S0 = ST + at * KT * 256 + turned_lane();
     const float* D0 = dST + at * KT * 256 + turned_lane();
     const float* U0 = UT + at * 4 * 256 + turned_lane();
-    const f32x4 br = turn4(at4(dUT + (at * 4 + wt) * 256 + turned_lane())), bu = turn4(at4(U0 + wt * 256));
+    const f32x4 br = at4(dUT + (at * 4 + wt) * 256 + tile_lane()), bu = turn4(at4(U0 + wt * 256));
 #pragma unroll
     for (int q = 0; q < KH; ++q)
       if (k0 + q < KT) {
@@ -215,6 +202,18 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
         X3[q] = mfma4(ds, bu, X3[q]);
         if ((q & 3) == wt) dot += s[0] * ds[0] + s[1] * ds[1] + s[2] * ds[2] + s[3] * ds[3];
       }
+    if ((vt & 1) == half) {
+      const f32x4 x = value4(v0, v), y = br * gt.beta[t];
+      rv += br[0] * x[0] + br[1] * x[1] + br[2] * x[2] + br[3] * x[3];
+      T* p = dv0 + (int64_t)t * cfg.dv_stride[1] + v;
+      if (t < rows) {
+        if (v + 4 <= d.V) store_pack<T, 4>(p, y);
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (v + e < d.V) p[e] = (T)y[e];
+      }
+    }
     const f32x4 bm = half ? br : bo;
 #pragma unroll
     for (int is = 0; is < 4; ++is)
@@ -222,6 +221,8 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   }
   dot = rowsum4(row16_sum(dot));
   if ((threadIdx.x & 63) == 0) dots[w] = dot;
+  rv = rowsum4(rv);
+  if (g == 0) dbv[half][t] = rv;
 #pragma unroll
   for (int is = 0; is < 4; ++is) {
 #pragma unroll
@@ -288,8 +289,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   if (w == 0) {
     const int l = threadIdx.x, seg = gt.seg[l];
     const float r = sums[0][1][l] + sums[1][1][l];
-    float db = r;
-    for (int i = 0; i < 8; ++i) db += dbv[i][l];
+    const float db = r + dbv[0][l] + dbv[1][l];
     if (l < rows) db0[(int64_t)l * cfg.dbeta_stride[1]] = l < a.nv ? db : 0.f;
     double end = (double)sums[0][3][l] + sums[1][3][l];
     double x = (double)sums[0][0][l] + sums[1][0][l] + gt.beta[l] * (double)r - sums[0][2][l] - sums[1][2][l] - end;
