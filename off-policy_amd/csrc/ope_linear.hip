@@ -15,6 +15,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_loose __attribute__((aligned(1)));
+typedef uint32_t u32_loose __attribute__((aligned(2)));
 
 template <typename T>
 __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c);
@@ -149,28 +150,120 @@ __device__ __forceinline__ void finish4(const Epilogue& e, f32x4 acc, int64_t m,
 
 struct Operand {
   const uint8_t* p;
-  int64_t rows, stride;            // stride in bytes
+  int64_t rows, stride;            // output rows this operand has; bytes from one row of memory to the next
 };
 
-// The tile kernel: BM x BN outputs a workgroup of 4 waves (2 x 2), 128 bytes of k a step, two LDS buffers: the next step's rows travel from
-// memory to registers while this step's are multiplied. 16-byte pieces are stored at piece ^ (row & 7), so neither the stores nor the 16-row
-// fragment reads collide in the banks. gridDim.y > 1: split of k; part [split][M][N] takes the sums and linear_join finishes.
-template <typename T, typename O, int BM, int BN>
-__global__ __launch_bounds__(256) void linear_tile(Operand A, Operand B, int64_t klen, int tiles_n, int steps_per, Epilogue e, float* __restrict__ part) {
-  constexpr int MT = BM / 32, NT = BN / 32, LA = BM / 32, LB = BN / 32;
-  __shared__ u32x4 As[2][BM][8], Bs[2][BN][8];
+// One operand's tile of R output rows and 128 bytes of the contraction, on its way from memory through registers to LDS (TH threads). LDS rows are 8
+// pieces of 16 bytes, stored at piece ^ (row & 7) so that neither the stores nor the 16-row fragment reads collide in the banks.
+//   ALONG: the contraction runs along memory; a thread moves whole pieces.
+//   else: it runs over the rows of memory (gradients: dz^T x, dz w); a thread takes C neighbouring columns of as many rows as a piece has elements and
+//   turns them in registers, so nothing is transposed in memory. 16 neighbouring lanes read one run of a row, the four rows of lanes behind them
+//   other pieces: their LDS stores then spread over all eight places.
+template <typename T, int R, int TH, bool ALONG>
+struct Loader {
+  static constexpr int N = R * 8 / TH;                                    // pieces a thread moves
+  static constexpr int E = 16 / (int)sizeof(T), C = N < 4 ? N : 4;        // elements of a piece; columns a thread takes
+  static constexpr int W = C * (int)sizeof(T) / 4;                        // 4-byte words of a row it takes
+  static_assert(R * 8 % TH == 0 && N % C == 0 && (ALONG || W >= 1), "tile and workgroup");
+  u32x4 r[N];
+  // Step s of the contraction. WHOLE: all of its 128 bytes are there, so no row of memory needs a check. Output rows past the last one read the last
+  // one's bytes again; what they make is not stored.
+  template <bool WHOLE>
+  __device__ __forceinline__ void fetch(const Operand& o, int64_t first, int64_t klen, int s) {
+    if constexpr (ALONG) {
+      const int row = threadIdx.x >> 3;
+      const int64_t k = (int64_t)s * 128 + (threadIdx.x & 7) * 16;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint8_t* p = o.p + min(first + row + TH / 8 * i, o.rows - 1) * o.stride;
+        r[i] = WHOLE ? *reinterpret_cast<const u32x4_loose*>(p + k) : row16(p, k, klen, (int)sizeof(T));
+      }
+    } else {
+      typedef uint32_t words __attribute__((ext_vector_type(W)));
+      typedef words words_loose __attribute__((aligned(2)));
+      const int64_t len = klen / (int)sizeof(T);                          // rows of memory
+#pragma unroll
+      for (int i = 0; i < N / C; ++i) {
+        const int x = threadIdx.x + TH * i, col = ((x & 15) + 16 * (x >> 7)) * C, piece = (x >> 4) & 7;
+        const int64_t n = first + col, m0 = (int64_t)s * (128 / (int)sizeof(T)) + piece * E;
+        const int here = (int)(n < o.rows ? min(o.rows - n, (int64_t)C) : 0);                        // columns of the C that exist
+        const uint8_t* p = o.p + m0 * o.stride + (here ? n : 0) * (int)sizeof(T);
+        uint32_t w[E][W];
+        if (WHOLE && (here == C || (here == 0 && o.rows >= C))) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const words v = *reinterpret_cast<const words_loose*>(p + e * o.stride);
+#pragma unroll
+            for (int c = 0; c < W; ++c) w[e][c] = ((const uint32_t*)&v)[c];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+#pragma unroll
+            for (int c = 0; c < W; ++c) w[e][c] = 0;
+            if (m0 + e < len)
+#pragma unroll
+              for (int c = 0; c < C; ++c)
+                if (c < here) {
+                  if (sizeof(T) == 4) w[e][c % W] = *reinterpret_cast<const uint32_t*>(p + e * o.stride + 4 * c);
+                  else w[e][c / 2 % W] |= (uint32_t) * reinterpret_cast<const uint16_t*>(p + e * o.stride + 2 * c) << (16 * (c % 2));
+                }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) r[C * i + c][e] = w[e][c];
+            else r[C * i + c][e] = __builtin_amdgcn_perm(w[2 * e + 1][c / 2], w[2 * e][c / 2], c % 2 ? 0x07060302 : 0x05040100);
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(u32x4 (*lds)[8]) const {
+    if constexpr (ALONG) {
+      const int row = threadIdx.x >> 3, piece = threadIdx.x & 7;
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds[row + TH / 8 * i][piece ^ (row & 7)] = r[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / C; ++i) {
+        const int x = threadIdx.x + TH * i, col = ((x & 15) + 16 * (x >> 7)) * C, piece = (x >> 4) & 7;
+#pragma unroll
+        for (int c = 0; c < C; ++c) lds[col + c][piece ^ ((col + c) & 7)] = r[C * i + c];
+      }
+    }
+  }
+};
+
+// The tile kernel: BM x BN outputs a workgroup of WM x WN waves, 128 bytes of k a step, two LDS buffers: the next step's rows travel from
+// memory to registers while this step's are multiplied. gridDim.y > 1: split of k; part [split][M][N] takes the sums and linear_join finishes.
+// Workgroups run over the XCDs in turn; each XCD gets one run of tiles, four rows of tiles high, so that its L2 sees few panels.
+template <typename T, typename O, int BM, int BN, int WM, int WN, bool AA, bool BA>
+__global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B, int64_t klen, int tiles_m, int tiles_n, int steps_per, Epilogue e,
+                                                            float* __restrict__ part) {
+  constexpr int TH = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+  __shared__ u32x4 lds[2 * (BM + BN) * 8];
+  u32x4(*As)[BM][8] = reinterpret_cast<u32x4(*)[BM][8]>(lds);
+  u32x4(*Bs)[BN][8] = reinterpret_cast<u32x4(*)[BN][8]>(lds + 2 * BM * 8);
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * BM, n0 = (int64_t)(blockIdx.x % tiles_n) * BN;
-  const int wm = (w >> 1) * (BM / 2), wn = (w & 1) * (BN / 2);
-  const int row = threadIdx.x >> 3, piece = threadIdx.x & 7;
+  const unsigned total = gridDim.x, per = total / 8, more = total % 8, xcd = blockIdx.x % 8;
+  const unsigned tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
+  const unsigned band = tile / (4u * tiles_n), high = min(4u, tiles_m - 4 * band), in = tile - band * 4u * tiles_n;
+  const int64_t m0 = (int64_t)(4 * band + in % high) * BM, n0 = (int64_t)(in / high) * BN;
+  const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
   const int steps = (int)((klen + 127) / 128), first = blockIdx.y * steps_per, last = min(first + steps_per, steps);
-  u32x4 ra[LA], rb[LB];
+  Loader<T, BM, TH, AA> la;
+  Loader<T, BN, TH, BA> lb;
+  const int whole = (int)(klen / 128);                 // steps without an end in them
   auto fetch = [&](int s) {
-    const int64_t k = (int64_t)s * 128 + piece * 16;
-#pragma unroll
-    for (int i = 0; i < LA; ++i) ra[i] = row16(A.p + min(m0 + row + 32 * i, A.rows - 1) * A.stride, k, klen, (int)sizeof(T));
-#pragma unroll
-    for (int i = 0; i < LB; ++i) rb[i] = row16(B.p + min(n0 + row + 32 * i, B.rows - 1) * B.stride, k, klen, (int)sizeof(T));
+    if (s < whole) {
+      la.template fetch<true>(A, m0, klen, s);
+      lb.template fetch<true>(B, n0, klen, s);
+    } else {
+      la.template fetch<false>(A, m0, klen, s);
+      lb.template fetch<false>(B, n0, klen, s);
+    }
   };
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -180,57 +273,72 @@ __global__ __launch_bounds__(256) void linear_tile(Operand A, Operand B, int64_t
   if (first < last) fetch(first);
   for (int s = first; s < last; ++s) {
     const int buf = (s - first) & 1;
-#pragma unroll
-    for (int i = 0; i < LA; ++i) As[buf][row + 32 * i][piece ^ (row & 7)] = ra[i];
-#pragma unroll
-    for (int i = 0; i < LB; ++i) Bs[buf][row + 32 * i][piece ^ (row & 7)] = rb[i];
+    la.store(As[buf]);
+    lb.store(Bs[buf]);
     lds_barrier();
     if (s + 1 < last) fetch(s + 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       u32x4 fa[MT], fb[NT];
 #pragma unroll
-      for (int a = 0; a < MT; ++a) fa[a] = As[buf][wm + 16 * a + j][(4 * h + g) ^ (j & 7)];
-#pragma unroll
       for (int b = 0; b < NT; ++b) fb[b] = Bs[buf][wn + 16 * b + j][(4 * h + g) ^ (j & 7)];
+#pragma unroll
+      for (int a = 0; a < MT; ++a) fa[a] = As[buf][wm + 16 * a + j][(4 * h + g) ^ (j & 7)];
 #pragma unroll
       for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = product<T>(fb[b], fa[a], acc[a][b]);
     }
   }
+  // The epilogue walks 16 rows at a time through the wave's own part of LDS: packs of whole rows leave (as the accumulators lie, a store would touch 16
+  // rows), and the code for a pack stands once for each 16 rows.
+  __syncthreads();
+  constexpr int CW = 16 * NT;                          // columns of a wave
+  float* mine = reinterpret_cast<float*>(lds) + w * 16 * (CW + 4);
 #pragma unroll
-  for (int a = 0; a < MT; ++a)
+  for (int a = 0; a < MT; ++a) {
 #pragma unroll
-    for (int b = 0; b < NT; ++b) {
-      const int64_t m = m0 + wm + 16 * a + j;
-      const int n = (int)n0 + wn + 16 * b + 4 * g;
-      if (gridDim.y == 1) finish4<O>(e, acc[a][b], m, n);
+    for (int b = 0; b < NT; ++b) *reinterpret_cast<f32x4*>(&mine[j * (CW + 4) + 16 * b + 4 * g]) = acc[a][b];
+#pragma unroll 1
+    for (int x = threadIdx.x & 63; x < 16 * CW / 4; x += 64) {
+      const int r = x / (CW / 4), c = x % (CW / 4) * 4, n = (int)n0 + wn + c;
+      const int64_t m = m0 + wm + 16 * a + r;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&mine[r * (CW + 4) + c]);
+      if (gridDim.y == 1) finish4<O>(e, v, m, n);
       else if (m < e.M && n < e.N) {
         float* p = part + ((int64_t)blockIdx.y * e.M + m) * e.N + n;
+        if (n + 4 <= e.N) store_pack<float, 4>(p, v);
+        else
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < e.N) p[r] = acc[a][b][r];
+          for (int i = 0; i < 4; ++i)
+            if (n + i < e.N) p[i] = v[i];
       }
     }
+  }
 }
 
-// Sums the splits in order and runs the epilogue.
+// Sums the splits and runs the epilogue: 16 packs of 4 outputs a workgroup, 16 runs of splits side by side and then in order.
 template <typename O>
 __global__ __launch_bounds__(256) void linear_join(const float* __restrict__ part, int splits, Epilogue e) {
-  const int per = ope_cdiv_dev4(e.N);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / per;
+  __shared__ f32x4 lds[16][17];
+  const int per = ope_cdiv_dev4(e.N), run = threadIdx.x >> 4;
+  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), m = i / per;
   const int n = (int)(i % per) * 4;
-  if (m >= e.M) return;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float* p = part + ((int64_t)s * e.M + m) * e.N + n;
-    if (n + 4 <= e.N) acc += load_pack<float, 4>(p);
-    else
+  if (m < e.M)
+    for (int s = run; s < splits; s += 16) {
+      const float* p = part + ((int64_t)s * e.M + m) * e.N + n;
+      if (n + 4 <= e.N) acc += load_pack<float, 4>(p);
+      else
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < e.N) acc[r] += p[r];
-  }
+        for (int r = 0; r < 4; ++r)
+          if (n + r < e.N) acc[r] += p[r];
+    }
+  lds[run][threadIdx.x & 15] = acc;
+  __syncthreads();
+  if (run) return;
+  acc = lds[0][threadIdx.x];
+  for (int r = 1; r < 16; ++r) acc += lds[r][threadIdx.x];
   finish4<O>(e, acc, m, n);
 }
 
@@ -267,38 +375,52 @@ __global__ __launch_bounds__(256) void linear_few(Operand A, Operand B, int64_t 
   }
 }
 
-// dz = dy act'(z) in tiles of 64 x 64: dz as it lies (where act' is not 1), its transpose [N][ldt], and the tile's column sums for dbias.
-// The same kernel transposes x and w (z = NULL, dz = NULL, no sums).
+// dz = dy act'(z), and the column sums of dz over a workgroup's kDzRows rows for dbias. 64 columns a workgroup; 4 neighbouring columns a lane, 16 rows side
+// by side. Without an activation (z = NULL) only the sums.
+constexpr int kDzRows = 256;
 template <typename T>
-__global__ __launch_bounds__(256) void linear_turn(const T* __restrict__ dy, int64_t stride, const T* __restrict__ z, int64_t M, int N, int act,
-                                                   T* __restrict__ dz, T* __restrict__ out, int64_t ldt, float* __restrict__ sums) {
-  __shared__ float tile[64][65];
-  const int tn = ope_cdiv_dev64(N);
-  const int64_t m0 = (int64_t)(blockIdx.x / tn) * 64;
-  const int n0 = (int)(blockIdx.x % tn) * 64;
-  for (int x = threadIdx.x; x < 64 * 64; x += 256) {
-    const int r = x >> 6, c = x & 63;
-    const int64_t m = m0 + r;
-    const int n = n0 + c;
-    float v = 0.f;
-    if (m < M && n < N) {
-      v = (float)dy[m * stride + n];
-      if (z) v *= act_slope((float)z[m * (int64_t)N + n], act);
-      if (dz) dz[m * (int64_t)N + n] = (T)v;
+__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const T* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
+                                                 float* __restrict__ sums) {
+  __shared__ f32x4 lds[16][17];
+  const int tn = ope_cdiv_dev64(N), n = (int)(blockIdx.x % tn) * 64 + (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
+  const int64_t m0 = (int64_t)(blockIdx.x / tn) * kDzRows;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (n < N)
+#pragma unroll 4
+    for (int r = r0; r < kDzRows; r += 16) {
+      const int64_t m = m0 + r, at = m * N + n;
+      if (m >= M) break;
+      f32x4 d = {0.f, 0.f, 0.f, 0.f}, x = d;
+      if (n + 4 <= N) {
+        d = load_pack<T, 4>(dy + at);
+        if (z) x = load_pack<T, 4>(z + at);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n + c < N) {
+            d[c] = (float)dy[at + c];
+            if (z) x[c] = (float)z[at + c];
+          }
+      }
+      if (z) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) d[c] *= act_slope(x[c], act);
+        if (n + 4 <= N) store_pack<T, 4>(dz + at, d);
+        else
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (n + c < N) dz[at + c] = (T)d[c];
+      }
+      s += d;
     }
-    tile[r][c] = v;
-  }
+  if (!sums) return;
+  lds[r0][threadIdx.x & 15] = s;
   __syncthreads();
-  if (out)
-    for (int x = threadIdx.x; x < 64 * 64; x += 256) {
-      const int c = x >> 6, r = x & 63;
-      if (n0 + c < N && m0 + r < M) out[(int64_t)(n0 + c) * ldt + m0 + r] = (T)tile[r][c];
-    }
-  if (sums && threadIdx.x < 64 && n0 + (int)threadIdx.x < N) {
-    float s = 0.f;
-    for (int r = 0; r < 64; ++r) s += tile[r][threadIdx.x];
-    sums[(int64_t)(blockIdx.x / tn) * N + n0 + threadIdx.x] = s;
-  }
+  if (r0 || n >= N) return;
+  for (int r = 1; r < 16; ++r) s += lds[r][threadIdx.x];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (n + c < N) sums[(int64_t)(blockIdx.x / tn) * N + n + c] = s[c];
 }
 template <typename T>
 __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ sums, int tiles, int N, T* __restrict__ out) {
@@ -316,13 +438,17 @@ __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ s
   }
 }
 
-// How one product is cut: tile size, and splits of k where the tiles alone leave CUs idle.
+// How one product is cut: the tile, and splits of k where the tiles alone leave CUs idle. Short contractions (under 8 steps of 128 bytes) and
+// small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least: a
+// round of 256 x 256 tiles (one a CU) is 4 units of work, one of 128 x 128 tiles (two a CU) 2 units at about 0.8 of the rate.
 struct Cut { int BM, tm, tn, steps, splits, per; bool few; };
 static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few) {
   Cut c;
   c.few = may_be_few && M <= 64;
   c.steps = (int)((klen + 127) / 128);
-  c.BM = (int64_t)ope_cdiv(M, 128) * ope_cdiv(N, 128) >= 256 ? 128 : 64;
+  const int64_t t128 = (int64_t)ope_cdiv(M, 128) * ope_cdiv(N, 128), t256 = (int64_t)ope_cdiv(M, 256) * ope_cdiv(N, 256);
+  c.BM = 64;
+  if (M > 64 && N > 64 && t128 >= 256 && c.steps >= 8) c.BM = 4.0 * ((t256 + 255) / 256) < 2.5 * ((t128 + 511) / 512) ? 256 : 128;
   c.tm = ope_cdiv(M, c.BM);
   c.tn = ope_cdiv(N, c.BM);
   const int64_t tiles = (int64_t)c.tm * c.tn;
@@ -339,24 +465,27 @@ static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few) {
 }
 static int64_t cut_floats(const Cut& c, int64_t M, int64_t N) { return c.splits > 1 ? (int64_t)c.splits * M * N : 0; }
 
-template <typename T, typename O>
-static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e, bool may_be_few, float* part, hipStream_t st) {
-  const Cut c = cut_of(e.M, e.N, klen, may_be_few);
-  if (c.few) {
-    const dim3 grid((unsigned)ope_cdiv(e.N, 16));
-    if (e.M <= 16) OPE_LAUNCH((linear_few<T, O, 1>), grid, dim3(256), 0, st, A, B, klen, e);
-    else if (e.M <= 32) OPE_LAUNCH((linear_few<T, O, 2>), grid, dim3(256), 0, st, A, B, klen, e);
-    else OPE_LAUNCH((linear_few<T, O, 4>), grid, dim3(256), 0, st, A, B, klen, e);
-    OPE_CHECK_LAUNCH();
-    return OPE_OK;
-  }
+// AA, BA: the contraction runs along memory in A / B
+template <typename T, typename O, bool AA, bool BA>
+static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e, float* part, hipStream_t st) {
+  const Cut c = cut_of(e.M, e.N, klen, AA && BA);
+  if constexpr (AA && BA)
+    if (c.few) {
+      const dim3 grid((unsigned)ope_cdiv(e.N, 16));
+      if (e.M <= 16) OPE_LAUNCH((linear_few<T, O, 1>), grid, dim3(256), 0, st, A, B, klen, e);
+      else if (e.M <= 32) OPE_LAUNCH((linear_few<T, O, 2>), grid, dim3(256), 0, st, A, B, klen, e);
+      else OPE_LAUNCH((linear_few<T, O, 4>), grid, dim3(256), 0, st, A, B, klen, e);
+      OPE_CHECK_LAUNCH();
+      return OPE_OK;
+    }
   const dim3 grid((unsigned)((int64_t)c.tm * c.tn), (unsigned)c.splits);
-  if (c.BM == 128) OPE_LAUNCH((linear_tile<T, O, 128, 128>), grid, dim3(256), 0, st, A, B, klen, c.tn, c.per, e, part);
-  else OPE_LAUNCH((linear_tile<T, O, 64, 64>), grid, dim3(256), 0, st, A, B, klen, c.tn, c.per, e, part);
+  if (c.BM == 256) OPE_LAUNCH((linear_tile<T, O, 256, 256, 2, 4, AA, BA>), grid, dim3(512), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
+  else if (c.BM == 128) OPE_LAUNCH((linear_tile<T, O, 128, 128, 2, 2, AA, BA>), grid, dim3(256), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
+  else OPE_LAUNCH((linear_tile<T, O, 64, 64, 2, 2, AA, BA>), grid, dim3(256), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
   OPE_CHECK_LAUNCH();
   if (c.splits > 1) {
     const int64_t n = e.M * ((e.N + 3) / 4);
-    OPE_LAUNCH((linear_join<O>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, c.splits, e);
+    OPE_LAUNCH((linear_join<O>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, c.splits, e);
     OPE_CHECK_LAUNCH();
   }
   return OPE_OK;
@@ -370,20 +499,16 @@ static bool linear_ok(const ope_linear_cfg* c) {
   return (int64_t)ope_cdiv(c->rows, 64) * ope_cdiv(c->out_width, 64) < ((int64_t)1 << 31) &&
          (int64_t)ope_cdiv(c->rows, 64) * ope_cdiv(c->in_width, 64) < ((int64_t)1 << 31);
 }
-static int64_t ld_of(int64_t rows) { return (rows + 15) & ~(int64_t)15; }     // rows of a transpose start on 16-byte pieces
 
-// What the backward pass needs beside its outputs, in elements of the type (e) and in floats (f)
-struct BwdPlan { int64_t dz, dzt, xt, wt, sums, part_dx, part_dw, bytes; };
+// What the backward pass needs beside its outputs, as offsets in bytes
+struct BwdPlan { int64_t dz, sums, part_dx, part_dw, bytes; };
 static BwdPlan bwd_plan(const ope_linear_cfg* c) {
   BwdPlan p;
   const int64_t M = c->rows, N = c->out_width, K = c->in_width, eb = elem_bytes(c->dtype);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t r = o; o += (bytes + 255) & ~(int64_t)255; return r; };
   p.dz = take(c->activation != OPE_ACT_NONE ? M * N * eb : 0);
-  p.dzt = take(N * ld_of(M) * eb);
-  p.xt = take(K * ld_of(M) * eb);
-  p.wt = take(K * ld_of(N) * eb);
-  p.sums = take((int64_t)ope_cdiv(M, 64) * N * 4);
+  p.sums = take((int64_t)ope_cdiv(M, kDzRows) * N * 4);
   p.part_dx = take(cut_floats(cut_of(M, K, N * eb, false), M, K) * 4);
   p.part_dw = take(cut_floats(cut_of(N, K, M * eb, false), N, K) * 4);
   p.bytes = o;
@@ -419,7 +544,7 @@ extern "C" int ope_linear(const ope_linear_cfg* cfg, const void* x, const void* 
   hipStream_t st = (hipStream_t)stream;
   return with_elem(cfg->out_dtype, [&](auto t) {
     typedef decltype(t) T;
-    return fp8 ? launch_product<e4m3_t, T>(A, B, klen, e, true, (float*)workspace, st) : launch_product<T, T>(A, B, klen, e, true, (float*)workspace, st);
+    return fp8 ? launch_product<e4m3_t, T, true, true>(A, B, klen, e, (float*)workspace, st) : launch_product<T, T, true, true>(A, B, klen, e, (float*)workspace, st);
   });
 }
 
@@ -447,12 +572,11 @@ extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, co
       OPE_CHECK_LAUNCH();
       return OPE_OK;
     }
-    const int tm = ope_cdiv(M, 64);
-    const int64_t ldm = ld_of(M), ldn = ld_of(N);
     const T* dz = acts ? (const T*)(ws + p.dz) : (const T*)dy;
-    if (acts || dw || dbias) {
-      OPE_LAUNCH((linear_turn<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(N, 64))), dim3(256), 0, st, (const T*)dy, (int64_t)N, acts ? (const T*)z : nullptr, M, N,
-                 cfg->activation, acts ? (T*)(ws + p.dz) : nullptr, dw ? (T*)(ws + p.dzt) : nullptr, ldm, dbias ? (float*)(ws + p.sums) : nullptr);
+    const int tm = ope_cdiv(M, kDzRows);
+    if (acts || dbias) {
+      OPE_LAUNCH((linear_dz<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(N, 64))), dim3(256), 0, st, (const T*)dy, acts ? (const T*)z : nullptr, M, N, cfg->activation,
+                 acts ? (T*)(ws + p.dz) : nullptr, dbias ? (float*)(ws + p.sums) : nullptr);
       OPE_CHECK_LAUNCH();
     }
     if (dbias) {
@@ -460,19 +584,15 @@ extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, co
       OPE_CHECK_LAUNCH();
     }
     if (dx) {
-      OPE_LAUNCH((linear_turn<T>), dim3((unsigned)((int64_t)ope_cdiv(N, 64) * ope_cdiv(K, 64))), dim3(256), 0, st, (const T*)w, (int64_t)K, (const T*)nullptr, (int64_t)N, K, 0,
-                 (T*)nullptr, (T*)(ws + p.wt), ldn, (float*)nullptr);
-      OPE_CHECK_LAUNCH();
       const Epilogue e = {nullptr, nullptr, nullptr, nullptr, dx, nullptr, 0, M, K, OPE_ACT_NONE};
-      const int rc = launch_product<T, T>({(const uint8_t*)dz, M, (int64_t)N * eb}, {ws + p.wt, K, ldn * eb}, (int64_t)N * eb, e, false, (float*)(ws + p.part_dx), st);
+      const int rc = launch_product<T, T, true, false>({(const uint8_t*)dz, M, (int64_t)N * eb}, {(const uint8_t*)w, K, (int64_t)K * eb}, (int64_t)N * eb, e,
+                                                       (float*)(ws + p.part_dx), st);
       if (rc) return rc;
     }
     if (dw) {
-      OPE_LAUNCH((linear_turn<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(K, 64))), dim3(256), 0, st, (const T*)x, cfg->x_stride, (const T*)nullptr, M, K, 0, (T*)nullptr,
-                 (T*)(ws + p.xt), ldm, (float*)nullptr);
-      OPE_CHECK_LAUNCH();
       const Epilogue e = {nullptr, nullptr, nullptr, nullptr, dw, nullptr, 0, N, K, OPE_ACT_NONE};
-      const int rc = launch_product<T, T>({ws + p.dzt, N, ldm * eb}, {ws + p.xt, K, ldm * eb}, M * eb, e, false, (float*)(ws + p.part_dw), st);
+      const int rc = launch_product<T, T, false, false>({(const uint8_t*)dz, N, (int64_t)N * eb}, {(const uint8_t*)x, K, cfg->x_stride * eb}, M * eb, e,
+                                                        (float*)(ws + p.part_dw), st);
       if (rc) return rc;
     }
     return OPE_OK;
