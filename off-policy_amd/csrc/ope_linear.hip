@@ -83,11 +83,14 @@ __device__ __forceinline__ u32x4 row16(const uint8_t* row, int64_t k, int64_t le
   return v;
 }
 
+// 1 / (1 + e^-z) by the hardware's 2^x and 1/x, each within one step of float32: with expf and a division the epilogue of a 4096 x 4096 output took
+// 20 us more than without an activation. e^-z past the range is infinite, its reciprocal 0.
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
 __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
     case OPE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
     case OPE_ACT_TANH: return tanhf(z);
-    case OPE_ACT_SILU: return z / (1.f + expf(-z));
+    case OPE_ACT_SILU: return z * sigmoid(z);
     case OPE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
   }
   return z;
@@ -96,7 +99,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case OPE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case OPE_ACT_TANH: { const float t = tanhf(z); return 1.f - t * t; }
-    case OPE_ACT_SILU: { const float s = 1.f / (1.f + expf(-z)); return s * (1.f + z * (1.f - s)); }
+    case OPE_ACT_SILU: { const float s = sigmoid(z); return s * (1.f + z * (1.f - s)); }
     case OPE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
   }
   return 1.f;

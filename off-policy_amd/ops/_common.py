@@ -80,6 +80,16 @@ def wants_grad(*ts):
     return False
 
 
+def once(backward):
+    """A backward pass that cannot be differentiated itself: refuses to be recorded (create_graph=True). torch's once_differentiable says it later,
+    at the second differentiation, at three times the cost for every call."""
+    def run(ctx, *grads):
+        if grad_enabled():
+            raise RuntimeError("the gradients of the memory operators cannot be differentiated again: no create_graph")
+        return backward(ctx, *grads)
+    return staticmethod(run)
+
+
 def size_or_raise(nbytes, what):
     """A negative size is the library's refusal of the configuration."""
     if nbytes < 0:

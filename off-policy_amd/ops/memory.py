@@ -3,10 +3,9 @@ import functools
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._common import PLANS, dtype_code, inner, like, on_device, ptr, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import PLANS, dtype_code, inner, like, on_device, once, ptr, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
 
 _CFG = struct.Struct("7if33q")
 _NONE3 = (0, 0, 0)
@@ -80,34 +79,35 @@ def _forward(plan, q, k, v, g, beta, state, lengths, scale):
 
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, lengths, scale, plan):
+    def forward(ctx, q, k, v, g, beta, state, lengths, call):
+        plan, scale = call
         o, last, saved = _forward(plan, q, k, v, g, beta, state, lengths, scale)
         ctx.save_for_backward(q, k, v, g, beta, lengths, saved)
-        ctx.scale, ctx.plan = scale, plan
+        ctx.call = call
         ctx.set_materialize_grads(False)
         return o, last
 
-    @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, do, dlast):
         if do is None and dlast is None:
-            return (None,) * 9
+            return (None,) * 8
         q, k, v, g, beta, lengths, saved = ctx.saved_tensors
-        B, _, H, _, K, V, _ = plan = ctx.plan
+        plan, scale = ctx.call
+        B, _, H, _, K, V, _ = plan
         with on_device(q, do, dlast):
             dev = q.device
             do = torch.zeros(v.shape, dtype=v.dtype, device=dev) if do is None else inner(do)
             dlast = None if dlast is None else dlast.contiguous()
             dq, dk, dv, dg, db = like(q), like(k), like(v), torch.empty_like(g), torch.empty_like(beta)
             dstate = torch.empty((B, H, K, V), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
-            cfg, saved_bytes, _, ws_bytes = _pack(plan, ctx.scale, q.stride(), k.stride(), v.stride(), do.stride(), g.stride(), beta.stride(), dq.stride(),
+            cfg, saved_bytes, _, ws_bytes = _pack(plan, scale, q.stride(), k.stride(), v.stride(), do.stride(), g.stride(), beta.stride(), dq.stride(),
                                                   dk.stride(), dv.stride(), dg.stride(), db.stride())
             hold, ws, _ = scratch(ws_bytes, dev)
             rc = _lib_backward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(saved), saved_bytes, do.data_ptr(),
                                ptr(dlast), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), db.data_ptr(), ptr(dstate), ws, ws_bytes, stream())
             if rc:
                 _lib.check(rc, "ope_delta_backward")
-        return dq, dk, dv, dg, db, dstate, None, None, None
+        return dq, dk, dv, dg, db, dstate, None, None
 
 
 def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None, scale=None):
@@ -131,7 +131,7 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
         state = None if initial_state is None else initial_state.contiguous()
         lengths = None if lengths is None else lengths.contiguous()
         if wants_grad(q, k, v, log_decay, beta, state):
-            return _GatedDelta.apply(q, k, v, log_decay, beta, state, lengths, scale, plan)
+            return _GatedDelta.apply(q, k, v, log_decay, beta, state, lengths, (plan, scale))
         return _forward(plan, q, k, v, log_decay, beta, state, lengths, scale)[:2]
 
 

@@ -3,10 +3,9 @@ import functools
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
 
 _CFG = struct.Struct("qqqiiif")
 _MAX_WIDTH = 1 << 20
@@ -71,20 +70,20 @@ def _forward(plan, x, weight, residual, eps, fp8, rstd_too):
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps, plan):
+    def forward(ctx, x, weight, residual, call):
+        plan, eps = call
         y, _, s, rstd = _forward(plan, x, weight, residual, eps, False, True)
         ctx.save_for_backward(x if s is None else s, weight, rstd)
-        ctx.eps, ctx.two, ctx.plan = eps, s is not None, plan
+        ctx.two, ctx.call = s is not None, call
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 
-    @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy, dsum=None):
         if dy is None and dsum is None:
-            return None, None, None, None, None
+            return None, None, None, None
         s, weight, rstd = ctx.saved_tensors
-        code, M, D = ctx.plan
+        (code, M, D), eps = ctx.call
         with on_device(s, dy, dsum):
             dev = s.device
             dy = torch.zeros(s.shape, dtype=s.dtype, device=dev) if dy is None else dy.contiguous()
@@ -92,13 +91,13 @@ class _RmsNorm(torch.autograd.Function):
             rows, xs = rows_of(s, D)
             dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
             dw = torch.empty(D, dtype=s.dtype, device=dev)
-            cfg = _pack(M, xs, 0, D, code, code, ctx.eps)
+            cfg = _pack(M, xs, 0, D, code, code, eps)
             hold, ws, nbytes = scratch(_bwd_bytes(cfg), dev)
             weight = weight.contiguous()
             rc = _lib_norm_bwd(cfg, dy.data_ptr(), ptr(dsum), rows.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws, nbytes, stream())
             if rc:
                 _lib.check(rc, "ope_rms_norm_backward")
-        return dx, dw, dx if ctx.two else None, None, None
+        return dx, dw, dx if ctx.two else None, None
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
@@ -111,7 +110,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     plan = _check(x, weight, residual, eps)
     with on_device(x, weight, residual):
         if wants_grad(x, weight, residual):
-            return _RmsNorm.apply(x, weight, residual, eps, plan)
+            return _RmsNorm.apply(x, weight, residual, (plan, eps))
         y, _, s, _ = _forward(plan, x, weight, residual, eps, False, False)
     return y if s is None else (y, s)
 

@@ -3,10 +3,9 @@ import functools
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
 
 ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "silu": 3, "gelu": 4}
 _CFG = struct.Struct("qqqiiiii4x")
@@ -85,8 +84,7 @@ class _Linear(torch.autograd.Function):
         ctx.plan = plan
         return y
 
-    @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         M, K, N, act, code, _ = ctx.plan
