@@ -136,6 +136,19 @@ __device__ __forceinline__ f32x4 column4(const T* p, int stride) {
   return v;
 }
 
+// Column `col` of a chunk of v or dO at the tokens 16 it + 4 g + r, it = 0..3: x[it][r], 0 outside the live tokens and the width. Every lane loads
+// (the nearest element inside where its own is outside): 16 loads in flight instead of 16 branches that each wait for one.
+template <typename T>
+__device__ __forceinline__ void load_columns(f32x4* x, const T* p, const int64_t* stride, const ChunkAt& a, int col, int V) {
+  const int g = (threadIdx.x >> 4) & 3;
+  const T* base = p + a.b * stride[0] + (int64_t)a.t0 * stride[1] + a.h * stride[2] + min(col, V - 1);
+  T raw[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) raw[i] = base[(int64_t)min(16 * (i >> 2) + 4 * g + (i & 3), a.nv - 1) * stride[1]];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = 16 * (i >> 2) + 4 * g + (i & 3) < a.nv && col < V ? (float)raw[i] : 0.f;
+}
+
 __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {   // 16 x 16 x 16: four steps of the f32 matrix instruction
 #pragma unroll
   for (int r = 0; r < 4; ++r) c = mfma16(a[r], b[r], c);

@@ -45,7 +45,6 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
     *reinterpret_cast<typename Pack<T, 4>::vec*>(KTs + (a.c * KT * 4 + x) * 256 + tile_lane()) = v;
   }
   __syncthreads();
-  const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)a.t0 * cfg.v_stride[1] + a.h * cfg.v_stride[2];
   for (int cg = w; cg < KT + d.VT; cg += NW) {
     f32x4 x[4];
     const int col = cg < KT ? 16 * cg + j : 16 * (cg - KT) + j;
@@ -53,15 +52,9 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
 #pragma unroll
       for (int it = 0; it < 4; ++it) x[it] = column4(&k.v[16 * it + 4 * g][col], Rows<T, KT>::kStride) * at4(&gt.head[16 * it + 4 * g]) * at4(&gt.beta[16 * it + 4 * g]);
     } else {
+load_columns(x, v_in, cfg.v_stride, a, col, d.V);
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = 16 * it + 4 * g + r;
-          x[it][r] = t < a.nv && col < d.V ? (float)v0[(int64_t)t * cfg.v_stride[1] + col] : 0.f;
-        }
-        x[it] *= at4(&gt.beta[16 * it + 4 * g]);
-      }
+      for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.beta[16 * it + 4 * g]);
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {

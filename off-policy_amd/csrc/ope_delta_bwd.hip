@@ -55,17 +55,10 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
     put4(&PT[s][16 * it + 4 * g], acc);
   }
   __syncthreads();
-  const T* o0 = dO + a.b * cfg.o_stride[0] + (int64_t)a.t0 * cfg.o_stride[1] + a.h * cfg.o_stride[2];
   for (int vt = w; vt < d.VT; vt += NW) {
     const int v = 16 * vt + j;
     f32x4 x[4];
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * it + 4 * g + r;
-        x[it][r] = t < a.nv && v < d.V ? (float)o0[(int64_t)t * cfg.o_stride[1] + v] : 0.f;
-      }
+    load_columns(x, dO, cfg.o_stride, a, v, d.V);
 #pragma unroll
     for (int is = 0; is < 4; ++is) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
