@@ -104,23 +104,35 @@ struct Rows {
   static constexpr int kStride = 16 * KT + 16 / (int)sizeof(T);
   T v[kC][kStride];
 };
-// What lies outside (tokens that are not live, columns past K) is 0.
-template <typename T, int KT>
+// What lies outside (tokens that are not live, columns past K) is 0. Lanes outside load the nearest row (and column) inside, so that all of a
+// thread's loads are in flight together. TH threads.
+template <typename T, int KT, int TH>
 __device__ __forceinline__ void load_rows(Rows<T, KT>& dst, const T* p, const int64_t* stride, const ChunkAt& a, int head, int K) {
   typedef typename Pack<T, 4>::vec vec;
+  constexpr int all = kC * KT * 4, N = (all + TH - 1) / TH;
   const T* base = p + a.b * stride[0] + (int64_t)a.t0 * stride[1] + head * stride[2];
-  for (int q = threadIdx.x; q < kC * KT * 4; q += blockDim.x) {
-    const int t = q / (KT * 4), k = (q % (KT * 4)) * 4;
-    vec v = (vec)(T)0.f;
-    if (t < a.nv) {
-      const T* row = base + (int64_t)t * stride[1];
-      if (k + 4 <= K) v = *reinterpret_cast<const typename Pack<T, 4>::loose*>(row + k);
-      else
+  vec v[N];
+  if (K == 16 * KT) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < K) v[e] = row[k + e];
+    for (int i = 0; i < N; ++i) {
+      const int q = min((int)threadIdx.x + TH * i, all - 1), t = q / (KT * 4), k = (q % (KT * 4)) * 4;
+      v[i] = *reinterpret_cast<const typename Pack<T, 4>::loose*>(base + (int64_t)min(t, a.nv - 1) * stride[1] + k);
     }
-    *reinterpret_cast<vec*>(&dst.v[t][k]) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int q = min((int)threadIdx.x + TH * i, all - 1), t = q / (KT * 4), k = (q % (KT * 4)) * 4;
+      const T* row = base + (int64_t)min(t, a.nv - 1) * stride[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = row[min(k + e, K - 1)];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int q = threadIdx.x + TH * i, t = q / (KT * 4), k = (q % (KT * 4)) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[i][e] = t < a.nv && k + e < K ? v[i][e] : (T)0.f;
+    if (q < all) *reinterpret_cast<vec*>(&dst.v[t][k]) = v[i];
   }
 }
 // four elements of a row / of a column, as float32

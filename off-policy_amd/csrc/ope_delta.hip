@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
   if (a.nv == 0) return;
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
-  load_rows(k, k_in, cfg.k_stride, a, a.h / (d.H / d.Hk), d.K);
+  load_rows<T, KT, 64 * NW>(k, k_in, cfg.k_stride, a, a.h / (d.H / d.Hk), d.K);
   __syncthreads();
   minus_A<T, KT>(NA, k, gt);
   if (threadIdx.x == 0) gC[a.c] = gt.whole;
@@ -229,8 +229,8 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(op
   fetch(0);
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
   const int hk = a.h / (d.H / d.Hk);
-  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows<T, KT, 256>(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows<T, KT, 256>(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
   const int t = 16 * w + j;
   f32x4 qs[KT], P[4];
@@ -251,7 +251,6 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(op
 #pragma unroll
   for (int c = 0; c < KT; ++c) qs[c] = row4(&q.v[t][16 * c + 4 * g]) * f;
   for (int vt = 0; vt < d.VT; ++vt) {
-    const int v = 16 * vt + j;
     f32x4 s1[KT], u1[4];
 #pragma unroll
     for (int c = 0; c < KT; ++c) s1[c] = s0[c];
@@ -265,10 +264,15 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(op
     for (int is = 0; is < 4; ++is)
       if (is <= w) acc2 = mfma4(P[is], u1[is], acc2);
     acc += acc2;
+    acc = turn4(acc);                      // four columns of one token a lane
+    const int tt = 16 * w + 4 * g + (j & 3), v4 = 16 * vt + 4 * (j >> 2);
+    if (tt < rows) {                       // (rows behind the last live token: q = 0, and so is this)
+      T* p = o0 + (int64_t)tt * cfg.o_stride[1] + v4;
+      if (v4 + 4 <= d.V) store_pack<T, 4>(p, acc);
+      else
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int tt = 16 * w + 4 * g + r;
-      if (tt < rows && v < d.V) o0[(int64_t)tt * cfg.o_stride[1] + v] = (T)(tt < a.nv ? acc[r] : 0.f);
+        for (int e = 0; e < 4; ++e)
+          if (v4 + e < d.V) p[e] = (T)acc[e];
     }
   }
 }

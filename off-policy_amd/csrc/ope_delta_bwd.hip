@@ -34,8 +34,8 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
   const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
   const int hk = a.h / (d.H / d.Hk);
-  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows<T, KT, 64 * NW>(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows<T, KT, 64 * NW>(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
   for (int x = w; x < 4 * KT; x += NW)                   // k, a tile a wave
     *reinterpret_cast<typename Pack<T, 4>::vec*>(Ks + (a.c * 4 * KT + x) * 256 + tile_lane()) =
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     return;
   }
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
-  load_rows(q, q_in, cfg.q_stride, a, hk, d.K);
-  load_rows(k, k_in, cfg.k_stride, a, hk, d.K);
+  load_rows<T, KT, 512>(q, q_in, cfg.q_stride, a, hk, d.K);
+  load_rows<T, KT, 512>(k, k_in, cfg.k_stride, a, hk, d.K);
   __syncthreads();
   minus_A<T, KT>(NA, k, gt);
   __syncthreads();
@@ -167,9 +167,13 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   const T* o0 = dO + a.b * cfg.o_stride[0] + (int64_t)(a.t0 + t) * cfg.o_stride[1] + a.h * cfg.o_stride[2];
   const T* v0 = v_in + a.b * cfg.v_stride[0] + (int64_t)(a.t0 + t) * cfg.v_stride[1] + a.h * cfg.v_stride[2];
   // four values of a row from column v on; nothing is read past the row's end or behind the last live token
-  auto value4 = [&](const T* row, int v) {
+  const int back = t - min(t, a.nv - 1);              // a token that is not live reads the last live one's row
+  auto value4 = [&](const T* row, int64_t stride, int v) {
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (t < a.nv) {
+    if (d.V == d.Vp) {
+      const f32x4 y = load_pack<T, 4>(row - back * stride + v);
+      x = back ? x : y;
+    } else if (t < a.nv) {
       if (v + 4 <= d.V) x = load_pack<T, 4>(row + v);
       else
 #pragma unroll
@@ -180,7 +184,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   };
   for (int vt = 0; vt < d.VT; ++vt) {
     const int v = 16 * vt + 4 * g;
-    const f32x4 bo = value4(o0, v);
+    const f32x4 bo = value4(o0, cfg.o_stride[1], v);
     const int64_t at = a.c * d.VT + vt;
     const float* S0 = ST + at * KT * 256 + turned_lane();
     const float* D0 = dST + at * KT * 256 + turned_lane();
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
         if ((q & 3) == wt) dot += s[0] * ds[0] + s[1] * ds[1] + s[2] * ds[2] + s[3] * ds[3];
       }
     if ((vt & 1) == half) {
-      const f32x4 x = value4(v0, v), y = br * gt.beta[t];
+      const f32x4 x = value4(v0, cfg.v_stride[1], v), y = br * gt.beta[t];
       rv += br[0] * x[0] + br[1] * x[1] + br[2] * x[2] + br[3] * x[3];
       T* p = dv0 + (int64_t)t * cfg.dv_stride[1] + v;
       if (t < rows) {
