@@ -715,11 +715,12 @@ int ope_rms_norm(const ope_norm_cfg* cfg, const void* x, const void* residual, c
                  float* rstd, void* stream);
 /* Gradients:  h = weight * dy;  dx = rstd * (h - s * rstd^2 * mean(h * s)) + dsum  (the residual's gradient is the same tensor),
  * dweight = sum over rows of dy * s * rstd, in a fixed order (no atomics).
- *   dy, s, dx [rows][width] contiguous of cfg->dtype (s: sum_out of the forward call, or x itself, row stride x_stride); dsum likewise or NULL;
- *   dweight [width] of cfg->dtype. dx may be dy or dsum. */
+ *   s = x + residual is formed again in float32 from the forward call's x and residual (or NULL), strides as there; float32 callers may pass sum_out for x
+ *   and no residual, which is the same sum. dy, dx and dsum (or NULL) [rows][width] contiguous of cfg->dtype; dweight [width] of cfg->dtype. dx may be
+ *   dy or dsum. */
 int64_t ope_rms_norm_backward_workspace_bytes(const ope_norm_cfg* cfg);
-int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd,
-                          void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* x, const void* residual, const void* weight,
+                          const float* rstd, void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 /* Rows of x in 8 bits with one scale each (the scale rule above), e.g. the weights of ope_linear with 8-bit operands. cfg->eps, out_dtype and
  * residual_stride are not read. */
 int ope_quantize_rows(const ope_norm_cfg* cfg, const void* x, void* q, float* scale, void* stream);
@@ -764,7 +765,8 @@ int ope_delta_step(const ope_delta_cfg* cfg, const void* q, const void* k, const
  *   contiguous, bias [out_width] and residual (rows residual_stride apart; bias / residual NULL = none) of out_dtype = dtype.
  *   dtype = OPE_E4M3: 8-bit x and w with x_scale [rows] and w_scale [out_width] float32, z = x_scale w_scale x w^T + bias; out_dtype is one of
  *   the other three. Forward only.
- *   z_out [rows][out_width] contiguous or NULL: z rounded to out_dtype, what the backward pass needs where activation is not OPE_ACT_NONE.
+ *   z_out [rows][out_width] contiguous or NULL: what the backward pass needs where activation is not OPE_ACT_NONE -- z in float32 (rounded to 16 bits it
+ *   would move act'(z) by more than the product's own rounding), for OPE_ACT_RELU, which asks for its sign alone, rounded to out_dtype.
  * Products are summed in float32. Backward: dz = dy act'(z), dx = dz w, dw = dz^T x, dbias = sum over rows of dz (the residual's gradient is dy);
  * dz is rounded to `dtype` for the products. dy, z contiguous; dx contiguous; dx, dw, dbias may be NULL (not wanted). Sums over rows are split in a
  * way that follows from the sizes alone and added in a fixed order. in_width, out_width 1..2^20, rows >= 0. */

@@ -209,7 +209,7 @@ def _load():
         # the operators' configurations travel as packed bytes (offpolicy_amd/ops/_common.py): a quarter of the cost of filling a ctypes struct
         "ope_rms_norm": (C.c_int, [p] * 9),
         "ope_rms_norm_backward_workspace_bytes": (i64, [p]),
-        "ope_rms_norm_backward": (C.c_int, [p] * 9 + [i64, p]),
+        "ope_rms_norm_backward": (C.c_int, [p] * 10 + [i64, p]),
         "ope_quantize_rows": (C.c_int, [p] * 5),
         "ope_delta_saved_bytes": (i64, [p]),
         "ope_delta_workspace_bytes": (i64, [p, i32]),

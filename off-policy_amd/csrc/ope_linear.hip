@@ -140,13 +140,15 @@ __device__ __forceinline__ void finish4(const Epilogue& e, f32x4 acc, int64_t m,
   const int64_t at = m * e.N + n;
   if (live == 4) {
     store_pack<O, 4>((O*)e.y + at, y);
-    if (e.z) store_pack<O, 4>((O*)e.z + at, z);
+    if (e.z && e.act == OPE_ACT_RELU) store_pack<O, 4>((O*)e.z + at, z);
+    else if (e.z) store_pack<float, 4>((float*)e.z + at, z);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (r < live) {
         ((O*)e.y)[at + r] = (O)y[r];
-        if (e.z) ((O*)e.z)[at + r] = (O)z[r];
+        if (e.z && e.act == OPE_ACT_RELU) ((O*)e.z)[at + r] = (O)z[r];
+        else if (e.z) ((float*)e.z)[at + r] = z[r];
       }
   }
 }
@@ -381,8 +383,8 @@ __global__ __launch_bounds__(256) void linear_few(Operand A, Operand B, int64_t 
 // dz = dy act'(z), and the column sums of dz over a workgroup's kDzRows rows for dbias. 64 columns a workgroup; 4 neighbouring columns a lane, 16 rows side
 // by side. Without an activation (z = NULL) only the sums.
 constexpr int kDzRows = 256;
-template <typename T>
-__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const T* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
+template <typename T, typename Z>
+__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const Z* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
                                                  float* __restrict__ sums) {
   __shared__ f32x4 lds[16][17];
   const int tn = ope_cdiv_dev64(N), n = (int)(blockIdx.x % tn) * 64 + (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const
       f32x4 d = {0.f, 0.f, 0.f, 0.f}, x = d;
       if (n + 4 <= N) {
         d = load_pack<T, 4>(dy + at);
-        if (z) x = load_pack<T, 4>(z + at);
+        if (z) x = load_pack<Z, 4>(z + at);
       } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -578,8 +580,11 @@ extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, co
     const T* dz = acts ? (const T*)(ws + p.dz) : (const T*)dy;
     const int tm = ope_cdiv(M, kDzRows);
     if (acts || dbias) {
-      OPE_LAUNCH((linear_dz<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(N, 64))), dim3(256), 0, st, (const T*)dy, acts ? (const T*)z : nullptr, M, N, cfg->activation,
-                 acts ? (T*)(ws + p.dz) : nullptr, dbias ? (float*)(ws + p.sums) : nullptr);
+      const dim3 grid((unsigned)((int64_t)tm * ope_cdiv(N, 64)));
+      T* out = acts ? (T*)(ws + p.dz) : nullptr;
+      float* sums = dbias ? (float*)(ws + p.sums) : nullptr;
+      if (cfg->activation == OPE_ACT_RELU) OPE_LAUNCH((linear_dz<T, T>), grid, dim3(256), 0, st, (const T*)dy, (const T*)z, M, N, cfg->activation, out, sums);
+      else OPE_LAUNCH((linear_dz<T, float>), grid, dim3(256), 0, st, (const T*)dy, acts ? (const float*)z : nullptr, M, N, cfg->activation, out, sums);
       OPE_CHECK_LAUNCH();
     }
     if (dbias) {

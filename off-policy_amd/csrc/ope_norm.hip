@@ -160,7 +160,7 @@ __global__ __launch_bounds__(1024) void norm_long(ope_norm_cfg c, const T* __res
 // [gridDim][nvec * VEC] and norm_dweight adds them in order. dx needs nothing but its own row.
 template <typename T, int VEC, int L, int NV>
 __global__ __launch_bounds__(L > 256 ? L : 256) void norm_bwd(ope_norm_cfg c, const T* dy, const T* dsum, const T* __restrict__ s_in,
-                                                              const T* __restrict__ weight, const float* __restrict__ rstd_in, T* dx,
+                                                              const T* __restrict__ residual, const T* __restrict__ weight, const float* __restrict__ rstd_in, T* dx,
                                                               float* __restrict__ part) {
   typedef typename Pack<T, VEC>::fvec fvec;
   constexpr int G = L > 256 ? 1 : 256 / L;             // rows a workgroup has in hand
@@ -186,6 +186,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void norm_bwd(ope_norm_cfg c, co
       s[n] = d[n] = (fvec)(0.f);
       if (on && i < nvec) {
         s[n] = load_pack<T, VEC>(s_in + row * c.x_stride + p);
+        if (residual) s[n] += load_pack<T, VEC>(residual + row * c.residual_stride + p);
         d[n] = load_pack<T, VEC>(dy + row * D + p);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
@@ -233,19 +234,20 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void norm_bwd(ope_norm_cfg c, co
 
 // The same for rows that do not fit: dweight's shares are added up in global memory, by the one workgroup and lane that owns the place.
 template <typename T>
-__global__ __launch_bounds__(1024) void norm_bwd_long(ope_norm_cfg c, const T* dy, const T* dsum, const T* __restrict__ s_in, const T* __restrict__ weight,
-                                                      const float* __restrict__ rstd_in, T* dx, float* __restrict__ part) {
+__global__ __launch_bounds__(1024) void norm_bwd_long(ope_norm_cfg c, const T* dy, const T* dsum, const T* __restrict__ s_in, const T* __restrict__ residual,
+                                                      const T* __restrict__ weight, const float* __restrict__ rstd_in, T* dx, float* __restrict__ part) {
   __shared__ float lds[16];
   const int D = c.width;
   float* mine = part + (int64_t)blockIdx.x * D;
+  auto at = [&](int64_t row, int d) { return (float)s_in[row * c.x_stride + d] + (residual ? (float)residual[row * c.residual_stride + d] : 0.f); };
   for (int d = threadIdx.x; d < D; d += 1024) mine[d] = 0.f;
   for (int64_t row = blockIdx.x; row < c.rows; row += gridDim.x) {
     const float rstd = rstd_in[row];
     float dot = 0.f;
-    for (int d = threadIdx.x; d < D; d += 1024) dot = fmaf((float)dy[row * D + d] * (float)weight[d], (float)s_in[row * c.x_stride + d], dot);
+    for (int d = threadIdx.x; d < D; d += 1024) dot = fmaf((float)dy[row * D + d] * (float)weight[d], at(row, d), dot);
     const float m = group_sum<1024>(dot, lds) / (float)D * rstd * rstd;
     for (int d = threadIdx.x; d < D; d += 1024) {
-      const float g = (float)dy[row * D + d], s = (float)s_in[row * c.x_stride + d];
+      const float g = (float)dy[row * D + d], s = at(row, d);
       mine[d] = fmaf(g, s * rstd, mine[d]);
       dx[row * D + d] = (T)(rstd * (g * (float)weight[d] - s * m) + (dsum ? (float)dsum[row * D + d] : 0.f));
     }
@@ -365,11 +367,11 @@ extern "C" int64_t ope_rms_norm_backward_workspace_bytes(const ope_norm_cfg* cfg
   return (int64_t)norm_parts(cfg) * (s.L ? s.nvec * s.VEC : cfg->width) * 4;
 }
 
-extern "C" int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* s_in, const void* weight, const float* rstd,
-                                     void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* x, const void* residual, const void* weight,
+                                     const float* rstd, void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
   const int64_t need = ope_rms_norm_backward_workspace_bytes(cfg);
-  if (need < 0 || !dweight) return OPE_EINVAL;
-  if (cfg->rows && (!dy || !s_in || !weight || !rstd || !dx || !workspace)) return OPE_EINVAL;
+  if (need < 0 || !dweight || (residual && cfg->residual_stride < 0)) return OPE_EINVAL;
+  if (cfg->rows && (!dy || !x || !weight || !rstd || !dx || !workspace)) return OPE_EINVAL;
   if (workspace_bytes < need) return OPE_ENOSPC;
   const NormShape s = norm_shape(cfg->dtype, cfg->width);
   const int parts = norm_parts(cfg), D = cfg->width, slots = s.L ? s.nvec * s.VEC : D;
@@ -381,13 +383,13 @@ extern "C" int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, co
     if (parts) {
       int rc = OPE_OK;
       if (s.L == 0)
-        OPE_LAUNCH((norm_bwd_long<T>), dim3(parts), dim3(1024), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)s_in, (const T*)weight, rstd, (T*)dx, part);
+        OPE_LAUNCH((norm_bwd_long<T>), dim3(parts), dim3(1024), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)x, (const T*)residual, (const T*)weight, rstd, (T*)dx, part);
       else if (s.VEC == 1)
-        OPE_LAUNCH((norm_bwd<T, 1, 16, 1>), dim3(parts), dim3(256), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)s_in, (const T*)weight, rstd, (T*)dx, part);
+        OPE_LAUNCH((norm_bwd<T, 1, 16, 1>), dim3(parts), dim3(256), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)x, (const T*)residual, (const T*)weight, rstd, (T*)dx, part);
       else
         rc = with_shape(s, [&](auto l, auto n) {
           constexpr int L = decltype(l)::value, NV = decltype(n)::value;
-          OPE_LAUNCH((norm_bwd<T, W, L, NV>), dim3(parts), dim3(L > 256 ? L : 256), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)s_in, (const T*)weight, rstd, (T*)dx, part);
+          OPE_LAUNCH((norm_bwd<T, W, L, NV>), dim3(parts), dim3(L > 256 ? L : 256), 0, st, *cfg, (const T*)dy, (const T*)dsum, (const T*)x, (const T*)residual, (const T*)weight, rstd, (T*)dx, part);
           return OPE_OK;
         });
       if (rc) return rc;

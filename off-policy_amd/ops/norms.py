@@ -73,7 +73,9 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, call):
         plan, eps = call
         y, _, s, rstd = _forward(plan, x, weight, residual, eps, False, True)
-        ctx.save_for_backward(x if s is None else s, weight, rstd)
+        # float32 keeps every bit of the sum; 16-bit types form it again from what was added
+        again = s is not None and x.dtype != torch.float32
+        ctx.save_for_backward(x if s is None or again else s, residual if again else None, weight, rstd)
         ctx.two, ctx.call = s is not None, call
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
@@ -82,19 +84,21 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, dy, dsum=None):
         if dy is None and dsum is None:
             return None, None, None, None
-        s, weight, rstd = ctx.saved_tensors
+        x, residual, weight, rstd = ctx.saved_tensors
         (code, M, D), eps = ctx.call
-        with on_device(s, dy, dsum):
-            dev = s.device
-            dy = torch.zeros(s.shape, dtype=s.dtype, device=dev) if dy is None else dy.contiguous()
+        with on_device(x, dy, dsum):
+            dev = x.device
+            dy = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dy is None else dy.contiguous()
             dsum = None if dsum is None else dsum.contiguous()
-            rows, xs = rows_of(s, D)
-            dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
-            dw = torch.empty(D, dtype=s.dtype, device=dev)
-            cfg = _pack(M, xs, 0, D, code, code, eps)
+            rows, xs = rows_of(x, D)
+            res, rs = (None, 0) if residual is None else rows_of(residual, D)
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            dw = torch.empty(D, dtype=x.dtype, device=dev)
+            cfg = _pack(M, xs, rs, D, code, code, eps)
             hold, ws, nbytes = scratch(_bwd_bytes(cfg), dev)
             weight = weight.contiguous()
-            rc = _lib_norm_bwd(cfg, dy.data_ptr(), ptr(dsum), rows.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws, nbytes, stream())
+            rc = _lib_norm_bwd(cfg, dy.data_ptr(), ptr(dsum), rows.data_ptr(), ptr(res), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws,
+                               nbytes, stream())
             if rc:
                 _lib.check(rc, "ope_rms_norm_backward")
         return dx, dw, dx if ctx.two else None, None
@@ -105,7 +109,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
     x [..., D] float32, bfloat16 or float16, weight [D] and residual (x's shape) of the same type. Returns y, or (y, s) where a residual is
     given: s is what the next block adds to. The norm is taken of the float32 sum, in front of its rounding to x's type. Differentiable in x,
-    weight and residual; the backward pass reads s as it was returned, so s must not be changed in place before it."""
+    weight and residual, once (no create_graph)."""
     eps = float(eps)
     plan = _check(x, weight, residual, eps)
     with on_device(x, weight, residual):

@@ -67,7 +67,7 @@ def _forward(plan, x, weight, x_scale, w_scale, bias, residual, out_dtype, keep_
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
-    z = torch.empty((M, N), dtype=out_dtype, device=dev) if keep_z else None
+    z = torch.empty((M, N), dtype=out_dtype if act == 1 else torch.float32, device=dev) if keep_z else None      # relu asks for z's sign alone
     cfg, need = _pack(M, xs, rs, K, N, code, out_code, act)
     hold, ws, nbytes = scratch(need, dev)
     rc = _lib_linear(cfg, rows.data_ptr(), weight.data_ptr(), ptr(x_scale), ptr(w_scale), ptr(bias), ptr(res), y.data_ptr(), ptr(z), ws, nbytes, stream())

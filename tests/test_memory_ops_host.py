@@ -112,8 +112,8 @@ def test_c_entries_check_before_they_launch():
     assert lib.ope_quantize_rows(norm(), some, some, None, some) == EINVAL
     need = lib.ope_rms_norm_backward_workspace_bytes(norm())
     assert need > 0 and lib.ope_rms_norm_backward_workspace_bytes(norm(width=0)) == EINVAL
-    assert lib.ope_rms_norm_backward(norm(), *[some] * 8, need - 1, some) == ENOSPC
-    assert lib.ope_rms_norm_backward(norm(), None, *[some] * 7, need, some) == EINVAL
+    assert lib.ope_rms_norm_backward(norm(), *[some] * 9, need - 1, some) == ENOSPC
+    assert lib.ope_rms_norm_backward(norm(), None, *[some] * 8, need, some) == EINVAL
 
     sizes = dict(batch=2, seq_len=5, n_heads=4, n_qk_heads=2, key_dim=8, value_dim=6)
     delta = lambda **k: C.byref(_lib.DeltaCfg(**{**sizes, **k}))                                                      # noqa: E731
