@@ -242,7 +242,8 @@ struct Loader {
 };
 
 // The tile kernel: BM x BN outputs a workgroup of WM x WN waves, 128 bytes of k a step, two LDS buffers: the next step's rows travel from
-// memory to registers while this step's are multiplied. gridDim.y > 1: split of k; part [split][M][N] takes the sums and linear_join finishes.
+// memory to registers while this step's are multiplied (two steps ahead took the second workgroup off the CU: 135 and 206 us instead of 96 and 103 in
+// the two products of 4096 x 2048 x 4096). gridDim.y > 1: split of k; part [split][M][N] takes the sums and linear_join finishes.
 // Workgroups run over the XCDs in turn; each XCD gets one run of tiles, four rows of tiles high, so that its L2 sees few panels.
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool AA, bool BA>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B, int64_t klen, int tiles_m, int tiles_n, int steps_per, Epilogue e,
@@ -347,35 +348,57 @@ __global__ __launch_bounds__(256) void linear_join(const float* __restrict__ par
   finish4<O>(e, acc, m, n);
 }
 
-// Few rows (up to 64): a workgroup has 16 columns, its four waves every fourth 64 bytes of k, straight from memory to the matrix instructions --
-// the weights are read once and by whole lines, and nothing waits for a barrier but the last sum over the waves.
+// Few rows (up to 64): a workgroup has 16 columns, its eight waves every eighth 64 bytes of k, straight from memory to the matrix instructions -- the
+// weights are read once and by whole lines, four loads of them in flight a wave, and nothing waits for a barrier but the last sum over the waves.
 template <typename T, typename O, int MT>
-__global__ __launch_bounds__(256) void linear_few(Operand A, Operand B, int64_t klen, Epilogue e) {
-  __shared__ float lds[4][MT][16][17];
-  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+__global__ __launch_bounds__(512) void linear_few(Operand A, Operand B, int64_t klen, Epilogue e) {
+  constexpr int NW = 8, D = 4;
+  __shared__ float lds[NW][MT][16][17];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const uint8_t* bp = B.p + min(n0 + j, B.rows - 1) * B.stride;
+  const uint8_t* bp = B.p + min(n0 + j, B.rows - 1) * B.stride + 16 * g;
   const uint8_t* ap[MT];
 #pragma unroll
-  for (int a = 0; a < MT; ++a) ap[a] = A.p + min((int64_t)16 * a + j, A.rows - 1) * A.stride;
+  for (int a = 0; a < MT; ++a) ap[a] = A.p + min((int64_t)16 * a + j, A.rows - 1) * A.stride + 16 * g;
   f32x4 acc[MT];
 #pragma unroll
   for (int a = 0; a < MT; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int64_t k0 = 64 * w; k0 < klen; k0 += 256) {
-    const int64_t k = k0 + 16 * g;
-    const u32x4 fb = row16(bp, k, klen, (int)sizeof(T));
+  int64_t k = 64 * w;
+  for (; k + 64 * NW * (D - 1) + 64 <= klen; k += 64 * NW * D) {
+    u32x4 fb[D], fa[D][MT];
 #pragma unroll
-    for (int a = 0; a < MT; ++a) acc[a] = product<T>(fb, row16(ap[a], k, klen, (int)sizeof(T)), acc[a]);
+    for (int i = 0; i < D; ++i) {
+      fb[i] = *reinterpret_cast<const u32x4_loose*>(bp + k + 64 * NW * i);
+#pragma unroll
+      for (int a = 0; a < MT; ++a) fa[i][a] = *reinterpret_cast<const u32x4_loose*>(ap[a] + k + 64 * NW * i);
+    }
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+      for (int a = 0; a < MT; ++a) acc[a] = product<T>(fb[i], fa[i][a], acc[a]);
+  }
+  for (; k < klen; k += 64 * NW) {
+    if (k + 64 <= klen) {
+      const u32x4 fb = *reinterpret_cast<const u32x4_loose*>(bp + k);
+#pragma unroll
+      for (int a = 0; a < MT; ++a) acc[a] = product<T>(fb, *reinterpret_cast<const u32x4_loose*>(ap[a] + k), acc[a]);
+    } else {
+      const u32x4 fb = row16(bp - 16 * g, k + 16 * g, klen, (int)sizeof(T));
+#pragma unroll
+      for (int a = 0; a < MT; ++a) acc[a] = product<T>(fb, row16(ap[a] - 16 * g, k + 16 * g, klen, (int)sizeof(T)), acc[a]);
+    }
   }
 #pragma unroll
   for (int a = 0; a < MT; ++a)
 #pragma unroll
     for (int r = 0; r < 4; ++r) lds[w][a][j][4 * g + r] = acc[a][r];
   __syncthreads();
-  for (int a = w; a < MT; a += 4) {
-    f32x4 v;
+  for (int a = w; a < MT; a += NW) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = ((lds[0][a][j][4 * g + r] + lds[1][a][j][4 * g + r]) + lds[2][a][j][4 * g + r]) + lds[3][a][j][4 * g + r];
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += lds[i][a][j][4 * g + r];
     finish4<O>(e, v, 16 * a + j, (int)n0 + 4 * g);
   }
 }
@@ -433,6 +456,7 @@ __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ s
   const int col = threadIdx.x & 63, run = threadIdx.x >> 6, n = blockIdx.x * 64 + col;
   float v = 0.f;
   if (n < N)
+#pragma unroll 8
     for (int r = run; r < tiles; r += 16) v += sums[(int64_t)r * N + n];
   lds[run][col] = v;
   __syncthreads();
@@ -477,9 +501,9 @@ static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e,
   if constexpr (AA && BA)
     if (c.few) {
       const dim3 grid((unsigned)ope_cdiv(e.N, 16));
-      if (e.M <= 16) OPE_LAUNCH((linear_few<T, O, 1>), grid, dim3(256), 0, st, A, B, klen, e);
-      else if (e.M <= 32) OPE_LAUNCH((linear_few<T, O, 2>), grid, dim3(256), 0, st, A, B, klen, e);
-      else OPE_LAUNCH((linear_few<T, O, 4>), grid, dim3(256), 0, st, A, B, klen, e);
+      if (e.M <= 16) OPE_LAUNCH((linear_few<T, O, 1>), grid, dim3(512), 0, st, A, B, klen, e);
+      else if (e.M <= 32) OPE_LAUNCH((linear_few<T, O, 2>), grid, dim3(512), 0, st, A, B, klen, e);
+      else OPE_LAUNCH((linear_few<T, O, 4>), grid, dim3(512), 0, st, A, B, klen, e);
       OPE_CHECK_LAUNCH();
       return OPE_OK;
     }

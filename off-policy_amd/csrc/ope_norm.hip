@@ -262,6 +262,7 @@ __global__ __launch_bounds__(1024) void norm_dweight(const float* __restrict__ p
   float v = 0.f;
   if (d < D) {
     const int last = slots - VEC, slot = d < last ? d : last + d - (D - VEC);
+#pragma unroll 8
     for (int r = run; r < parts; r += 16) v += part[(int64_t)r * slots + slot];
   }
   lds[run][col] = v;
