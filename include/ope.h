@@ -691,7 +691,8 @@ int ope_allreduce_flat_dev(const ope_allreduce_ctx* ctx_host, uint32_t* epoch_st
 /* ------------------------------------------------------------------------------------------------
  * Memory-block operators: what an agent with a wider or longer memory than the GRU of rnn.py:5-43 is made of. Each takes float32, bfloat16 or
  * float16 tensors (OPE_F32 / OPE_BF16 / OPE_F16), computes in float32 and rounds once where it stores. No entry allocates, synchronises or
- * keeps anything between calls; workspaces are the caller's, and a call may be recorded into a HIP graph.
+ * keeps anything between calls; workspaces are the caller's, and a call may be recorded into a HIP graph. Sizes whose launch would hold 2^32 threads
+ * or more return OPE_EINVAL.
  * ---------------------------------------------------------------------------------------------- */
 #define OPE_F32 0
 #define OPE_BF16 1
@@ -765,8 +766,8 @@ int ope_delta_step(const ope_delta_cfg* cfg, const void* q, const void* k, const
  *   contiguous, bias [out_width] and residual (rows residual_stride apart; bias / residual NULL = none) of out_dtype = dtype.
  *   dtype = OPE_E4M3: 8-bit x and w with x_scale [rows] and w_scale [out_width] float32, z = x_scale w_scale x w^T + bias; out_dtype is one of
  *   the other three. Forward only.
- *   z_out [rows][out_width] contiguous or NULL: what the backward pass needs where activation is not OPE_ACT_NONE -- z in float32 (rounded to 16 bits it
- *   would move act'(z) by more than the product's own rounding), for OPE_ACT_RELU, which asks for its sign alone, rounded to out_dtype.
+ *   z_out float32 [rows][out_width] contiguous or NULL: z, what the backward pass needs where activation is not OPE_ACT_NONE (rounded to 16 bits it
+ *   would move act'(z) by more than the product's own rounding).
  * Products are summed in float32. Backward: dz = dy act'(z), dx = dz w, dw = dz^T x, dbias = sum over rows of dz (the residual's gradient is dy);
  * dz is rounded to `dtype` for the products. dy, z contiguous; dx contiguous; dx, dw, dbias may be NULL (not wanted). Sums over rows are split in a
  * way that follows from the sizes alone and added in a fixed order. in_width, out_width 1..2^20, rows >= 0. */
@@ -781,9 +782,9 @@ typedef struct ope_linear_cfg {
 } ope_linear_cfg;
 int64_t ope_linear_workspace_bytes(const ope_linear_cfg* cfg);
 int ope_linear(const ope_linear_cfg* cfg, const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
-               const void* residual, void* y, void* z_out, void* workspace, int64_t workspace_bytes, void* stream);
+               const void* residual, void* y, float* z_out, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t ope_linear_backward_workspace_bytes(const ope_linear_cfg* cfg);
-int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, const void* z, const void* x, const void* w, void* dx, void* dw, void* dbias,
+int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, const float* z, const void* x, const void* w, void* dx, void* dw, void* dbias,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

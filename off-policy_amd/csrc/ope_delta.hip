@@ -12,7 +12,9 @@ bool delta_ok(const ope_delta_cfg* c) {
   if (!c || c->batch < 0 || c->seq_len < 0 || c->n_heads < 1 || c->n_qk_heads < 1 || c->n_heads % c->n_qk_heads) return false;
   if (c->key_dim < 1 || c->key_dim > 128 || c->value_dim < 1 || c->value_dim > 1024 || !elem_float(c->dtype)) return false;
   const DeltaDims d = delta_dims(c);
-  return (int64_t)d.B * d.H * (d.n > d.VT ? d.n : d.VT) < ((int64_t)1 << 31);     // workgroups of one launch
+  const int64_t bh = (int64_t)d.B * d.H;                // (below 2^62; so are the products, each factor being checked first)
+  if (!launch_fits(bh, 512) || !launch_fits(bh * d.VT, 256) || !launch_fits(bh * d.n, 512) || !launch_fits(bh * d.K * d.V / 256 + 1, 256)) return false;
+  return d.H == d.Hk || launch_fits((int64_t)d.B * d.T * d.Hk * d.K / 256 + 1, 256);
 }
 
 // Rows of one chunk-head: W = (I + A)^-1 beta e^G k, U0 = (I + A)^-1 beta v by block forward substitution, 16 columns a wave at a time.

@@ -27,6 +27,9 @@ __device__ __forceinline__ void store_pack(T* p, typename Pack<T, N>::fvec f) {
   *reinterpret_cast<typename Pack<T, N>::loose*>(p) = __builtin_convertvector(f, typename Pack<T, N>::vec);
 }
 
+// A launch holds fewer than 2^32 threads; what would pass that is refused with the arguments, not left to the runtime.
+static inline bool launch_fits(int64_t blocks, int threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 static inline int elem_bytes(int dtype) { return dtype == OPE_F32 ? 4 : (dtype == OPE_E4M3 ? 1 : 2); }
 static inline bool elem_float(int dtype) { return dtype == OPE_F32 || dtype == OPE_BF16 || dtype == OPE_F16; }
 

@@ -108,7 +108,8 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 struct Epilogue {
   const float *x_scale, *w_scale;
   const void *bias, *residual;
-  void *y, *z;
+  void* y;
+  float* z;
   int64_t residual_stride;
   int64_t M;
   int N, act;
@@ -140,15 +141,13 @@ __device__ __forceinline__ void finish4(const Epilogue& e, f32x4 acc, int64_t m,
   const int64_t at = m * e.N + n;
   if (live == 4) {
     store_pack<O, 4>((O*)e.y + at, y);
-    if (e.z && e.act == OPE_ACT_RELU) store_pack<O, 4>((O*)e.z + at, z);
-    else if (e.z) store_pack<float, 4>((float*)e.z + at, z);
+    if (e.z) store_pack<float, 4>(e.z + at, z);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (r < live) {
         ((O*)e.y)[at + r] = (O)y[r];
-        if (e.z && e.act == OPE_ACT_RELU) ((O*)e.z)[at + r] = (O)z[r];
-        else if (e.z) ((float*)e.z)[at + r] = z[r];
+        if (e.z) e.z[at + r] = z[r];
       }
   }
 }
@@ -406,8 +405,8 @@ __global__ __launch_bounds__(512) void linear_few(Operand A, Operand B, int64_t 
 // dz = dy act'(z), and the column sums of dz over a workgroup's kDzRows rows for dbias. 64 columns a workgroup; 4 neighbouring columns a lane, 16 rows side
 // by side. Without an activation (z = NULL) only the sums.
 constexpr int kDzRows = 256;
-template <typename T, typename Z>
-__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const Z* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
+template <typename T>
+__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const float* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
                                                  float* __restrict__ sums) {
   __shared__ f32x4 lds[16][17];
   const int tn = ope_cdiv_dev64(N), n = (int)(blockIdx.x % tn) * 64 + (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
@@ -421,13 +420,13 @@ __global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const
       f32x4 d = {0.f, 0.f, 0.f, 0.f}, x = d;
       if (n + 4 <= N) {
         d = load_pack<T, 4>(dy + at);
-        if (z) x = load_pack<Z, 4>(z + at);
+        if (z) x = load_pack<float, 4>(z + at);
       } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           if (n + c < N) {
             d[c] = (float)dy[at + c];
-            if (z) x[c] = (float)z[at + c];
+            if (z) x[c] = z[at + c];
           }
       }
       if (z) {
@@ -525,8 +524,8 @@ static bool linear_ok(const ope_linear_cfg* c) {
   if (c->in_width > (1 << 20) || c->out_width > (1 << 20) || c->x_stride < 0 || c->residual_stride < 0) return false;
   if (c->activation < OPE_ACT_NONE || c->activation > OPE_ACT_GELU || !elem_float(c->out_dtype)) return false;
   if (c->dtype != OPE_E4M3 && (!elem_float(c->dtype) || c->dtype != c->out_dtype)) return false;
-  return (int64_t)ope_cdiv(c->rows, 64) * ope_cdiv(c->out_width, 64) < ((int64_t)1 << 31) &&
-         (int64_t)ope_cdiv(c->rows, 64) * ope_cdiv(c->in_width, 64) < ((int64_t)1 << 31);
+  const int64_t tm = ope_cdiv(c->rows, 64), tn = ope_cdiv(c->out_width, 64), tk = ope_cdiv(c->in_width, 64);
+  return launch_fits(tm * tn, 256) && launch_fits(tm * tk, 256) && launch_fits(tn * tk * 16, 256);      // (16: the fill of dw where there are no rows)
 }
 
 // What the backward pass needs beside its outputs, as offsets in bytes
@@ -559,7 +558,7 @@ extern "C" int64_t ope_linear_workspace_bytes(const ope_linear_cfg* cfg) {
 }
 
 extern "C" int ope_linear(const ope_linear_cfg* cfg, const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
-                          const void* residual, void* y, void* z_out, void* workspace, int64_t workspace_bytes, void* stream) {
+                          const void* residual, void* y, float* z_out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!linear_ok(cfg)) return OPE_EINVAL;
   if (cfg->rows == 0) return OPE_OK;
   const bool fp8 = cfg->dtype == OPE_E4M3;
@@ -582,7 +581,7 @@ extern "C" int64_t ope_linear_backward_workspace_bytes(const ope_linear_cfg* cfg
   return bwd_plan(cfg).bytes;
 }
 
-extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, const void* z, const void* x, const void* w, void* dx, void* dw, void* dbias,
+extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, const float* z, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                    void* workspace, int64_t workspace_bytes, void* stream) {
   if (!linear_ok(cfg) || cfg->dtype == OPE_E4M3) return OPE_EINVAL;
   const int64_t M = cfg->rows;
@@ -604,11 +603,8 @@ extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, co
     const T* dz = acts ? (const T*)(ws + p.dz) : (const T*)dy;
     const int tm = ope_cdiv(M, kDzRows);
     if (acts || dbias) {
-      const dim3 grid((unsigned)((int64_t)tm * ope_cdiv(N, 64)));
-      T* out = acts ? (T*)(ws + p.dz) : nullptr;
-      float* sums = dbias ? (float*)(ws + p.sums) : nullptr;
-      if (cfg->activation == OPE_ACT_RELU) OPE_LAUNCH((linear_dz<T, T>), grid, dim3(256), 0, st, (const T*)dy, (const T*)z, M, N, cfg->activation, out, sums);
-      else OPE_LAUNCH((linear_dz<T, float>), grid, dim3(256), 0, st, (const T*)dy, acts ? (const float*)z : nullptr, M, N, cfg->activation, out, sums);
+      OPE_LAUNCH((linear_dz<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(N, 64))), dim3(256), 0, st, (const T*)dy, acts ? z : nullptr, M, N, cfg->activation,
+                 acts ? (T*)(ws + p.dz) : nullptr, dbias ? (float*)(ws + p.sums) : nullptr);
       OPE_CHECK_LAUNCH();
     }
     if (dbias) {

@@ -311,9 +311,10 @@ static int with_shape(const NormShape& s, F f) {
 }
 
 static bool norm_ok(const ope_norm_cfg* c) {
-  if (!c || c->rows < 0 || c->width < 1 || c->width > (1 << 20) || !elem_float(c->dtype)) return false;
-  if (c->rows > ((int64_t)1 << 31) - 1 || c->x_stride < 0) return false;
-  return true;
+  if (!c || c->rows < 0 || c->width < 1 || c->width > (1 << 20) || !elem_float(c->dtype) || c->x_stride < 0) return false;
+  const NormShape s = norm_shape(c->dtype, c->width);
+  const int lanes = s.L ? s.L : 1024;                  // of one row
+  return c->rows < ((int64_t)1 << 31) && launch_fits(c->rows + 16, lanes);
 }
 
 template <bool NORM, bool OUT8>

@@ -123,7 +123,8 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
     the rule needs beta |k|^2 < 2 to stay bounded.
 
     Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 at -inf), beta and
-    initial_state. The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32: (K V + 64 (K + V)) * 4 bytes."""
+    initial_state, once (no create_graph). The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32:
+    (K V + 64 (K + V)) * 4 bytes."""
     plan = _check(q, k, v, log_decay, beta, initial_state, lengths, 2)
     scale = float(plan[4] ** -0.5 if scale is None else scale)
     with on_device(q, k, v, log_decay, beta, initial_state, lengths):

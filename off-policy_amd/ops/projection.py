@@ -67,7 +67,7 @@ def _forward(plan, x, weight, x_scale, w_scale, bias, residual, out_dtype, keep_
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
-    z = torch.empty((M, N), dtype=out_dtype if act == 1 else torch.float32, device=dev) if keep_z else None      # relu asks for z's sign alone
+    z = torch.empty((M, N), dtype=torch.float32, device=dev) if keep_z else None
     cfg, need = _pack(M, xs, rs, K, N, code, out_code, act)
     hold, ws, nbytes = scratch(need, dev)
     rc = _lib_linear(cfg, rows.data_ptr(), weight.data_ptr(), ptr(x_scale), ptr(w_scale), ptr(bias), ptr(res), y.data_ptr(), ptr(z), ws, nbytes, stream())
@@ -114,7 +114,7 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     """y = act(x weight^T + bias) + residual.
 
     x [..., in], weight [out, in] (torch.nn.Linear's), bias [out], residual [..., out], all of one type (float32, bfloat16 or float16); activation
-    "none", "relu", "tanh", "silu" or "gelu" (z Phi(z)). Sums in float32, one rounding at the end. Differentiable in all four; the gradient of
+    "none", "relu", "tanh", "silu" or "gelu" (z Phi(z)). Sums in float32, one rounding at the end. Differentiable in all four, once (no create_graph); the gradient of
     z = x weight^T + bias is rounded to x's type in front of the backward products."""
     tensors((x, "x"))
     dtype_code(x.dtype, "x")

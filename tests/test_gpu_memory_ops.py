@@ -268,11 +268,9 @@ def test_norm_and_its_gradients(ops, D, dtype):
         want = torch.autograd.grad([y64, s64] if residual else [y64], wide, [dy.double(), ds.double()] if residual else [dy.double()])
         rstd = (s64.detach().square().mean(-1, keepdim=True) + 1e-5).rsqrt()
         size = ((wide[1].abs() * dy.double().abs()).max() * rstd.max() * 2).item() + (ds.abs().max().item() if residual else 0)
-        # s reaches the backward pass rounded to its type: each of dx's two terms moves by up to a half step of it more, at the terms' size
-        extra = size * R.half_step(dtype) * 2 / R.U32 if residual and dtype != F32 else 0
-        R.close(grads[0], want[0], 1, 16 + D ** 0.5 + extra / size, "dx", size)
+        R.close(grads[0], want[0], 1, 16 + D ** 0.5, "dx", size)
         part = (dy.double() * s64.detach() * rstd).abs().sum(0).max().item()
-        R.close(grads[1], want[1], 1, M + 16 + (R.half_step(dtype) / R.U32 if residual and dtype != F32 else 0), "dweight", part)
+        R.close(grads[1], want[1], 1, M + 16, "dweight", part)
         if residual:
             assert torch.equal(grads[0], grads[2])
         with torch.no_grad():
@@ -293,9 +291,8 @@ def test_norm_of_rows_past_the_registers(ops, dtype):
     R.close(y.detach(), y64.detach(), 1, 64, "y")
     R.close(s.detach(), s64.detach(), 1, 1, "s")
     dy = randn(g, 3, D, dtype=dtype)
-    extra = 2 * R.half_step(dtype) / R.U32 if dtype != F32 else 0
     for name, a, b in zip(("dx", "dw", "dr"), torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y64, wide, dy.double())):
-        R.close(a, b, 1, 64 + extra, name, 2 * b.abs().max().item())
+        R.close(a, b, 1, 64, name, 2 * b.abs().max().item())
     with torch.no_grad():
         check_fp8(*ops.rms_norm_fp8(x, w, residual=r)[:2], y64.detach())
 
@@ -402,10 +399,8 @@ def check_linear(ops, g, M, K, N, dtype, act, bias=True, residual=True, x=None):
     dy = randn(g, M, N, dtype=dtype)
     got = dict(zip(args, torch.autograd.grad(y, leaves, dy)))
     want = dict(zip(args, torch.autograd.grad(y64, list(wide.values()), dy.double())))
-    # dz = dy act'(z) is rounded to its type once more, and so is the z it is taken at (act'' is at most 1 in all of these); the relu's slope jumps where
-    # z is within its error of 0: inputs whose z comes that close are left out of the comparison by giving them no gradient
-    z64 = (wide["x"] @ wide["weight"].t() + (wide["bias"] if bias else 0)).detach()
-    more = (R.half_step(dtype) * (1 + (1 if act != "none" else 0) * z64.abs().max().item()) / R.U32 if dtype != F32 else 0) + K + 8
+    # dz = dy act'(z) is rounded to its type in front of the products
+    more = (R.half_step(dtype) / R.U32 if dtype != F32 else 0) + K + 8
     d = dy.double().abs()
     sizes = {"x": (d @ w.double().abs()).max().item() if M else 0, "weight": (d.t() @ x.double().abs()).max().item() if M else 0, "bias": d.sum(0).max().item() if M else 0}
     terms = {"x": N, "weight": M, "bias": M}
@@ -476,7 +471,7 @@ def test_linear_gradients_that_are_not_wanted(ops):
 
 
 @pytest.mark.parametrize("out", [F32, BF16, F16])
-@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (5, 40, 33), (16, 256, 512), (64, 2048, 96), (65, 130, 70), (300, 512, 260), (2050, 128, 2050)])
+@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (5, 40, 33), (16, 256, 512), (64, 2048, 96), (65, 130, 70), (300, 512, 260), (2050, 128, 2050), (20, 37, 45), (70, 333, 129)])
 def test_linear_on_8_bits(ops, M, K, N, out):
     g = gen(36)
     xq, xs = ops.quantize_rows_fp8(randn(g, M, K))
@@ -661,6 +656,32 @@ def test_the_same_call_gives_the_same_bits(ops):
     first = torch.autograd.grad(ops.linear(x, w, activation="silu"), [x, w], dy)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(ops.linear(x, w, activation="silu"), [x, w], dy)))
+
+
+def test_gradients_twice_from_one_graph_and_never_of_gradients(ops):
+    """retain_graph gives the same bits again; a graph of the gradients themselves is refused, not silently wrong."""
+    g = gen(46)
+    block = Block(g, 32, 2, 16, 16, BF16)
+    leaves = [t.detach().requires_grad_() for t in (randn(g, 2, 70, 32, dtype=BF16), randn(g, 2, 70, 32, dtype=BF16), *block.p)]
+    y, _ = block(ops, leaves[0], leaves[1], leaves[2:])
+    dy = randn(g, 2, 70, 32, dtype=BF16)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, dy)))
+    x, w = randn(g, 4, 8).requires_grad_(), randn(g, 8).requires_grad_()
+    for out in (ops.rms_norm(x, w), ops.linear(x, randn(g, 5, 8)), ops.gated_delta_rule(*[t.requires_grad_() for t in delta_inputs(g, 1, 3, 1, 1, 4, 4, F32)])[0]):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out.sum(), x if out.shape != (1, 3, 1, 4) else out, create_graph=True) if out.shape != (1, 3, 1, 4) else out.sum().backward(create_graph=True)
+
+
+def test_changed_inputs_are_noticed(ops):
+    """What the backward pass reads and somebody changed in between is an error, as everywhere in torch."""
+    g = gen(47)
+    for dtype in (F32, BF16):
+        x, w, r = randn(g, 4, 8, dtype=dtype).requires_grad_(), randn(g, 8, dtype=dtype).requires_grad_(), randn(g, 4, 8, dtype=dtype)
+        y, s = ops.rms_norm(x, w, residual=r)
+        (s.detach() if dtype == F32 else r).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
 
 
 def test_tensors_on_two_devices_are_refused(ops):

@@ -104,7 +104,7 @@ def test_c_entries_check_before_they_launch():
     norm = lambda **k: C.byref(_lib.NormCfg(**{**dict(rows=2, x_stride=8, width=8, eps=1e-6), **k}))                  # noqa: E731
     some = C.c_void_p(16)                                     # never dereferenced: every call below is refused first
     assert lib.ope_rms_norm(None, *[some] * 8) == EINVAL
-    for k in (dict(width=0), dict(rows=-1), dict(dtype=3), dict(dtype=7), dict(out_dtype=1), dict(eps=-1.0), dict(eps=float("nan")), dict(x_stride=-8), dict(width=(1 << 20) + 1)):
+    for k in (dict(width=0), dict(rows=-1), dict(dtype=3), dict(dtype=7), dict(out_dtype=1), dict(eps=-1.0), dict(eps=float("nan")), dict(x_stride=-8), dict(width=(1 << 20) + 1), dict(rows=1 << 31), dict(rows=1 << 28), dict(rows=1 << 23, width=8192)):
         assert lib.ope_rms_norm(norm(**k), *[some] * 8) == EINVAL, k
     assert lib.ope_rms_norm(norm(), None, *[some] * 7) == EINVAL
     assert lib.ope_rms_norm(norm(out_dtype=3), some, some, some, some, None, some, some, some) == EINVAL      # 8 bits without a place for the scales
@@ -118,7 +118,8 @@ def test_c_entries_check_before_they_launch():
     sizes = dict(batch=2, seq_len=5, n_heads=4, n_qk_heads=2, key_dim=8, value_dim=6)
     delta = lambda **k: C.byref(_lib.DeltaCfg(**{**sizes, **k}))                                                      # noqa: E731
     for k in (dict(batch=-1), dict(seq_len=-1), dict(n_heads=0), dict(n_qk_heads=0), dict(n_qk_heads=3), dict(key_dim=0), dict(key_dim=129), dict(value_dim=0),
-              dict(value_dim=1025), dict(dtype=3), dict(batch=1 << 20, n_heads=1 << 12, seq_len=1 << 20)):
+              dict(value_dim=1025), dict(dtype=3), dict(batch=1 << 20, n_heads=1 << 12, seq_len=1 << 20), dict(batch=1 << 30, n_heads=1 << 30),
+              dict(batch=1 << 22), dict(batch=1 << 14, seq_len=1 << 14, n_heads=4, key_dim=128)):
         assert lib.ope_delta_saved_bytes(delta(**k)) == EINVAL and lib.ope_delta_workspace_bytes(delta(**k), 1) == EINVAL, k
         assert lib.ope_delta_forward(delta(**k), *[some] * 10, 1 << 40, some, 1 << 40, some) == EINVAL, k
         assert lib.ope_delta_step(delta(**k), *[some] * 8) == EINVAL, k
@@ -135,7 +136,7 @@ def test_c_entries_check_before_they_launch():
 
     lin = lambda **k: C.byref(_lib.LinearCfg(**{**dict(rows=100, x_stride=8, in_width=8, out_width=5), **k}))          # noqa: E731
     for k in (dict(rows=-1), dict(in_width=0), dict(out_width=0), dict(in_width=(1 << 20) + 1), dict(dtype=1), dict(dtype=3, out_dtype=3), dict(dtype=9), dict(activation=5),
-              dict(activation=-1), dict(x_stride=-1), dict(rows=1 << 31)):
+              dict(activation=-1), dict(x_stride=-1), dict(rows=1 << 31), dict(rows=1 << 30, out_width=1 << 14), dict(in_width=1 << 20, out_width=1 << 13)):
         assert lib.ope_linear_workspace_bytes(lin(**k)) == EINVAL and lib.ope_linear(lin(**k), *[some] * 9, 1 << 40, some) == EINVAL, k
     assert lib.ope_linear(lin(), some, some, some, None, *[some] * 5, 1 << 40, some) == EINVAL                  # scales are for 8-bit operands
     assert lib.ope_linear(lin(dtype=3), some, some, some, None, *[some] * 5, 1 << 40, some) == EINVAL
