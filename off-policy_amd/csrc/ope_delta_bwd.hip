@@ -79,8 +79,7 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
 }
 
 // Eight waves: wave w owns the tokens 16 (w & 3).. as data rows and one half (w >> 2) of the key tiles, so the three products over the value
-// columns keep 3 * KT / 2 accumulators in registers and S, dS' are read by four waves instead of eight. The first half makes dP, the second
-// dA; they change hands through LDS, where dP takes the place of A once the triangular solve is done.
+// columns keep 3 * KT / 2 accumulators in registers. The first half makes dP, the second dA; they change hands through LDS.
 template <typename T, int KT>
 __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_main(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
                                                       const T* __restrict__ v_in, const float* __restrict__ g_in, const float* __restrict__ beta_in,
@@ -90,12 +89,19 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
                                                       float* __restrict__ dg, float* __restrict__ dbeta) {
   constexpr int RS = Rows<T, KT>::kStride, KH = (KT + 1) / 2;      // KH: key tiles of a half
   __shared__ Rows<T, KT> q, k;
-  __shared__ float NA[kC][kC + 4], dAs[kC][kC + 4], inv[4][16][20];
+  // One pool, three lives: A and the diagonal's inverses for the solve; the tiles of S, dS' and U of 16 columns (rows of 20 floats: stores of whole
+  // lanes and reads along columns both spread over the banks); dP and dA.
+  constexpr int kTiles = 2 * KT + 4, kTile = 16 * 20, kPool = 2 * kC * (kC + 4) + 4 * 16 * 20;
+  static_assert(kTiles * kTile <= kPool, "LDS pool");
+  __shared__ float pool[kPool];
+  float(*NA)[kC + 4] = reinterpret_cast<float(*)[kC + 4]>(pool);
+  float(*dPs)[kC + 4] = NA;
+  float(*dAs)[kC + 4] = reinterpret_cast<float(*)[kC + 4]>(pool + kC * (kC + 4));
+  float(*inv)[16][20] = reinterpret_cast<float(*)[16][20]>(pool + 2 * kC * (kC + 4));
   __shared__ float dbv[2][kC], sums[2][4][kC], dots[8];
   __shared__ Gates gt;
-  float(*dPs)[kC + 4] = NA;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
-  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   const int rows = min(d.T - a.t0, kC), hk = a.h / (d.H / d.Hk);
   const bool own = d.H == d.Hk;
   T* dv0 = dv + a.b * cfg.dv_stride[0] + (int64_t)a.t0 * cfg.dv_stride[1] + a.h * cfg.dv_stride[2];
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     }
   }
   __syncthreads();     // dR of all columns is in dUT; A is done with
-  const int wt = w & 3, half = w >> 2, k0 = half * KH, t = 16 * wt + j;
+  const int wt = __builtin_amdgcn_readfirstlane(w & 3), half = __builtin_amdgcn_readfirstlane(w >> 2), k0 = half * KH, t = 16 * wt + j;
   f32x4 X1[KH], X2[KH], X3[KH], M[4];
 #pragma unroll
   for (int q = 0; q < KH; ++q) X1[q] = X2[q] = X3[q] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -182,26 +188,50 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     }
     return x;
   };
+  // The tiles of 16 columns reach LDS once (each wave loads its share of the next ones while these are multiplied) and are read from there
+  // transposed: 334 us at 4 x 4096 x 8 x 128 x 128. Loaded by the waves that multiply them, four times over, they kept the L2 at 7 TB/s: 420 us.
+  constexpr int kShare = (kTiles + 7) / 8;
+  f32x4 pre[kShare], br, bo;
+  const int64_t first = a.c * d.VT;
+  auto fetch = [&](int vt) {                           // past the end: the last columns again
+    const int64_t at = first + min(vt, d.VT - 1);
+    const int v = 16 * min(vt, d.VT - 1) + 4 * g;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+      const int x = min(w + 8 * i, kTiles - 1);
+      const float* p = x < KT ? ST + (at * KT + x) * 256 : (x < 2 * KT ? dST + (at * KT + x - KT) * 256 : UT + (at * 4 + x - 2 * KT) * 256);
+      pre[i] = at4(p + tile_lane());
+    }
+    br = at4(dUT + (at * 4 + wt) * 256 + tile_lane());
+    bo = value4(o0, cfg.o_stride[1], v);
+  };
+  auto tile = [&](int x) { return col4(&pool[x * kTile + 4 * g * 20 + j], 20); };
+  fetch(0);
   for (int vt = 0; vt < d.VT; ++vt) {
     const int v = 16 * vt + 4 * g;
-    const f32x4 bo = value4(o0, cfg.o_stride[1], v);
-    const int64_t at = a.c * d.VT + vt;
-    const float* S0 = ST + at * KT * 256 + turned_lane();
-    const float* D0 = dST + at * KT * 256 + turned_lane();
-    const float* U0 = UT + at * 4 * 256 + turned_lane();
-    const f32x4 br = at4(dUT + (at * 4 + wt) * 256 + tile_lane()), bu = turn4(at4(U0 + wt * 256));
+#pragma unroll
+    for (int i = 0; i < kShare; ++i)
+      if (w + 8 * i < kTiles) put4(&pool[(w + 8 * i) * kTile + j * 20 + 4 * g], pre[i]);
+    const f32x4 r = br, o = bo, x = value4(v0, cfg.v_stride[1], v);
+    lds_barrier();
+    fetch(vt + 1);
+    const f32x4 bu = tile(2 * KT + wt), bm = half ? r : o;
 #pragma unroll
     for (int q = 0; q < KH; ++q)
-      if (k0 + q < KT) {
-        const f32x4 s = turn4(at4(S0 + (k0 + q) * 256)), ds = turn4(at4(D0 + (k0 + q) * 256));
-        X1[q] = mfma4(s, bo, X1[q]);
-        X2[q] = mfma4(s, br, X2[q]);
-        X3[q] = mfma4(ds, bu, X3[q]);
-        if ((q & 3) == wt) dot += s[0] * ds[0] + s[1] * ds[1] + s[2] * ds[2] + s[3] * ds[3];
+      if (KT % 2 == 0 || k0 + q < KT) {
+        const f32x4 st = tile(k0 + q), dt = tile(KT + k0 + q);
+        X1[q] = mfma4(st, o, X1[q]);
+        X2[q] = mfma4(st, r, X2[q]);
+        X3[q] = mfma4(dt, bu, X3[q]);
+        if ((q & 3) == wt) dot += st[0] * dt[0] + st[1] * dt[1] + st[2] * dt[2] + st[3] * dt[3];
+        if (q & 1) __builtin_amdgcn_sched_barrier(0);  // no more tiles in registers than two pairs: 128 are what two workgroups a CU leave
       }
-    if ((vt & 1) == half) {
-      const f32x4 x = value4(v0, cfg.v_stride[1], v), y = br * gt.beta[t];
-      rv += br[0] * x[0] + br[1] * x[1] + br[2] * x[2] + br[3] * x[3];
+#pragma unroll
+    for (int is = 0; is < 4; ++is)
+      if (is <= wt) M[is] = mfma4(tile(2 * KT + is), bm, M[is]);
+    if ((vt & 1) == half) {                            // one half writes dv and counts dR.v
+      const f32x4 y = r * gt.beta[t];
+      rv += r[0] * x[0] + r[1] * x[1] + r[2] * x[2] + r[3] * x[3];
       T* p = dv0 + (int64_t)t * cfg.dv_stride[1] + v;
       if (t < rows) {
         if (v + 4 <= d.V) store_pack<T, 4>(p, y);
@@ -211,10 +241,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
             if (v + e < d.V) p[e] = (T)y[e];
       }
     }
-    const f32x4 bm = half ? br : bo;
-#pragma unroll
-    for (int is = 0; is < 4; ++is)
-      if (is <= wt) M[is] = mfma4(turn4(at4(U0 + is * 256)), bm, M[is]);
+    lds_barrier();
   }
   dot = rowsum4(row16_sum(dot));
   if ((threadIdx.x & 63) == 0) dots[w] = dot;
