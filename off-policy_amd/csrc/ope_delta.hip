@@ -205,28 +205,34 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
 }
 
 // o of one chunk-head. Wave w owns the tokens 16w..: its rows of scale tril(q k^T decay) and of scale e^G q stay in registers while it walks
-// the value columns; S and U of the next 16 columns are loaded while these are multiplied.
+// the value columns. The tiles of S and U of 16 columns reach LDS once, in two buffers where q and k were: each wave loads a quarter of the next ones
+// while these are multiplied.
 template <typename T, int KT>
-__global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
+__global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 4) void delta_out(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in,
                                                  const float* __restrict__ g_in, const float* __restrict__ beta_in, const int32_t* __restrict__ lengths,
                                                  const float* __restrict__ ST, const float* __restrict__ UT, T* __restrict__ o) {
-  __shared__ Rows<T, KT> k, q;
+  constexpr int kTiles = KT + 4, kShare = (kTiles + 3) / 4;
+  constexpr int kRows = 2 * (int)sizeof(Rows<T, KT>), kStage = 2 * kTiles * 1024;
+  __shared__ __attribute__((aligned(16))) uint8_t pool[kRows > kStage ? kRows : kStage];
+  Rows<T, KT>&k = reinterpret_cast<Rows<T, KT>*>(pool)[0], &q = reinterpret_cast<Rows<T, KT>*>(pool)[1];
+  float* stage = reinterpret_cast<float*>(pool);
   __shared__ Gates gt;
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
-  const int w = threadIdx.x >> 6, j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   T* o0 = o + a.b * cfg.o_stride[0] + (int64_t)a.t0 * cfg.o_stride[1] + a.h * cfg.o_stride[2];
   const int rows = min(d.T - a.t0, kC);
   if (a.nv == 0) {
     for (int e = threadIdx.x; e < rows * d.V; e += 256) o0[(int64_t)(e / d.V) * cfg.o_stride[1] + e % d.V] = (T)0.f;
     return;
   }
-  f32x4 s0[KT], u0[4];
-  auto fetch = [&](int vt) {
-    const int64_t at = a.c * d.VT + vt;
+  f32x4 pre[kShare];
+  auto fetch = [&](int vt) {                           // past the end: the last columns again
+    const int64_t at = a.c * d.VT + min(vt, d.VT - 1);
 #pragma unroll
-    for (int c = 0; c < KT; ++c) s0[c] = at4(&ST[(at * KT + c) * 256 + tile_lane()]);
-#pragma unroll
-    for (int is = 0; is < 4; ++is) u0[is] = at4(&UT[(at * 4 + min(is, w)) * 256 + tile_lane()]);
+    for (int i = 0; i < kShare; ++i) {
+      const int x = min(w + 4 * i, kTiles - 1);
+      pre[i] = at4((x < KT ? ST + (at * KT + x) * 256 : UT + (at * 4 + x - KT) * 256) + tile_lane());
+    }
   };
   fetch(0);
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
@@ -252,19 +258,20 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 3) void delta_out(op
   const float f = cfg.scale * gt.head[t];
 #pragma unroll
   for (int c = 0; c < KT; ++c) qs[c] = row4(&q.v[t][16 * c + 4 * g]) * f;
+  __syncthreads();                                     // q and k are done with
   for (int vt = 0; vt < d.VT; ++vt) {
-    f32x4 s1[KT], u1[4];
+    float* tiles = stage + (vt & 1) * kTiles * 256 + tile_lane();
 #pragma unroll
-    for (int c = 0; c < KT; ++c) s1[c] = s0[c];
-#pragma unroll
-    for (int is = 0; is < 4; ++is) u1[is] = u0[is];
-    if (vt + 1 < d.VT) fetch(vt + 1);
+    for (int i = 0; i < kShare; ++i)
+      if (w + 4 * i < kTiles) put4(tiles + (w + 4 * i) * 256, pre[i]);
+    lds_barrier();
+    fetch(vt + 1);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
 #pragma unroll
-    for (int c = 0; c < KT; ++c) acc = mfma4(qs[c], s1[c], acc);
+    for (int c = 0; c < KT; ++c) acc = mfma4(qs[c], at4(tiles + c * 256), acc);
 #pragma unroll
     for (int is = 0; is < 4; ++is)
-      if (is <= w) acc2 = mfma4(P[is], u1[is], acc2);
+      if (is <= w) acc2 = mfma4(P[is], at4(tiles + (KT + is) * 256), acc2);
     acc += acc2;
     acc = turn4(acc);                      // four columns of one token a lane
     const int tt = 16 * w + 4 * g + (j & 3), v4 = 16 * vt + 4 * (j >> 2);
