@@ -691,7 +691,7 @@ int ope_allreduce_flat_dev(const ope_allreduce_ctx* ctx_host, uint32_t* epoch_st
 /* ------------------------------------------------------------------------------------------------
  * Memory-block operators: what an agent with a wider or longer memory than the GRU of rnn.py:5-43 is made of. Each takes float32, bfloat16 or
  * float16 tensors (OPE_F32 / OPE_BF16 / OPE_F16), computes in float32 and rounds once where it stores. No entry allocates, synchronises or
- * keeps anything between calls; workspaces are the caller's, and a call may be recorded into a HIP graph. Sizes whose launch would hold 2^32 threads
+ * keeps anything between calls; workspaces are the caller's, outputs overlap no inputs, and a call may be recorded into a HIP graph. Sizes whose launch would hold 2^32 threads
  * or more return OPE_EINVAL.
  * ---------------------------------------------------------------------------------------------- */
 #define OPE_F32 0
@@ -704,7 +704,7 @@ int ope_allreduce_flat_dev(const ope_allreduce_ctx* ctx_host, uint32_t* epoch_st
  *   weight       [width] of `dtype`
  *   y            [rows][width] contiguous, of `dtype` -- or, with out_dtype = OPE_E4M3, 8-bit values of y / scale[row],
  *                scale[row] = max(max|y|, 448 * 2^-126) / 448 (float32; NaN where the row holds one)
- *   sum_out      [rows][width] contiguous, s rounded to `dtype`; NULL = not wanted. May be `x` or `residual` itself where that is contiguous.
+ *   sum_out      [rows][width] contiguous, s rounded to `dtype`; NULL = not wanted
  *   rstd         float32 [rows], 1 / sqrt(mean(s^2) + eps) for the backward pass; NULL = not wanted
  * The norm is taken of the unrounded float32 sum. rows >= 0, 1 <= width <= 2^20. */
 typedef struct ope_norm_cfg {
@@ -717,8 +717,7 @@ int ope_rms_norm(const ope_norm_cfg* cfg, const void* x, const void* residual, c
 /* Gradients:  h = weight * dy;  dx = rstd * (h - s * rstd^2 * mean(h * s)) + dsum  (the residual's gradient is the same tensor),
  * dweight = sum over rows of dy * s * rstd, in a fixed order (no atomics).
  *   s = x + residual is formed again in float32 from the forward call's x and residual (or NULL), strides as there; float32 callers may pass sum_out for x
- *   and no residual, which is the same sum. dy, dx and dsum (or NULL) [rows][width] contiguous of cfg->dtype; dweight [width] of cfg->dtype. dx may be
- *   dy or dsum. */
+ *   and no residual, which is the same sum. dy, dx and dsum (or NULL) [rows][width] contiguous of cfg->dtype; dweight [width] of cfg->dtype. */
 int64_t ope_rms_norm_backward_workspace_bytes(const ope_norm_cfg* cfg);
 int ope_rms_norm_backward(const ope_norm_cfg* cfg, const void* dy, const void* dsum, const void* x, const void* residual, const void* weight,
                           const float* rstd, void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream);

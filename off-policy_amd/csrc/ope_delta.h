@@ -7,14 +7,15 @@
 //
 // Arrays in `saved` (S, kept for the backward pass) and in the workspace (W). All lie in TILES of 16 x 16, in the order in which the lanes of a
 // wave hold them: lane (j, g) has row j, columns 4g .. 4g+3, tile after tile, so that every access of a wave is one run of whole cache lines (rows
-// of the matrices themselves took twice the time: a CU's requests in flight, not its bytes, bound the scan). turn4 gives a tile transposed.
-//   ST  [c][VT][KT]  float32 S  the state in front of the chunk: rows v, columns k       (a tile index is the last two indexes)
-//   UT  [c][VT][4]   float32 S  u of the chunk's tokens (U0 before the scan): rows v, columns t
-//   WT  [c][KT][4]   float32 S  W transposed: rows k, columns t
-//   gC  [c]          float32 S  decay over the whole chunk (0 behind a reset);  tails [c][64] float32 S  decay from t to the chunk's end
-//   W   [c][4][KT]   float32 W  rows t, columns k                                KTs [c][KT][4] of the inputs' type W  k transposed: rows k, columns t
-//   backward: Ks [c][4][KT] of the inputs' type W (rows t, columns k), dUT like UT (dU0, then dU, then dR with its tiles transposed), dST like ST (N, then the gradient of the
-//   state BEHIND the chunk), dqp, dkp [b][t][H][K] float32 where query / key heads are shared
+// of the matrices themselves took twice the time: a CU's requests in flight, not its bytes, bound the scan). turn4 gives a tile transposed. The
+// last two indexes below count tiles; float32 unless said otherwise.
+//   ST [c][VT][KT]  S  the state in front of the chunk: rows v, columns k
+//   UT [c][VT][4]   S  U0 before the scan, u of the chunk's tokens after it: rows v, columns t
+//   WT [c][KT][4]   S  W transposed: rows k, columns t
+//   gC [c]          S  decay over the whole chunk (0 behind a reset);   tails [c][64]  S  decay from t to the chunk's end
+//   W  [c][4][KT]   W  rows t, columns k;   KTs [c][KT][4]  W  of the inputs' type: k transposed, rows k, columns t
+//   backward: Ks [c][4][KT]  W  of the inputs' type: k, rows t, columns k;   dUT like UT (dU0, then dU, then dR with its tiles transposed);
+//   dST like ST (N, then the gradient of the state BEHIND the chunk);   dqp, dkp [b][t][H][K] where query / key heads are shared
 #pragma once
 #include <type_traits>
 

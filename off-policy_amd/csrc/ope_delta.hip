@@ -19,8 +19,8 @@ bool delta_ok(const ope_delta_cfg* c) {
 
 // Rows of one chunk-head: W = (I + A)^-1 beta e^G k, U0 = (I + A)^-1 beta v by block forward substitution, 16 columns a wave at a time.
 template <typename T, int KT>
-__global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ k_in, const T* __restrict__ v_in,
-                                                                    const float* __restrict__ g_in, const float* __restrict__ beta_in,
+__global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta_prep(ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ k_in,
+                                                                    const T* __restrict__ v_in, const float* __restrict__ g_in, const float* __restrict__ beta_in,
                                                                     const int32_t* __restrict__ lengths, float* __restrict__ W, float* __restrict__ WT,
                                                                     T* __restrict__ KTs, float* __restrict__ UT, float* __restrict__ gC,
                                                                     float* __restrict__ tails) {
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
 #pragma unroll
       for (int it = 0; it < 4; ++it) x[it] = column4(&k.v[16 * it + 4 * g][col], Rows<T, KT>::kStride) * at4(&gt.head[16 * it + 4 * g]) * at4(&gt.beta[16 * it + 4 * g]);
     } else {
-load_columns(x, v_in, cfg.v_stride, a, col, d.V);
+      load_columns(x, v_in, cfg.v_stride, a, col, d.V);
 #pragma unroll
       for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.beta[16 * it + 4 * g]);
     }

@@ -204,7 +204,6 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void norm_bwd(ope_norm_cfg c, co
       out[n] = rstd * (d[n] * w[n] - s[n] * m);
       if (on && i < nvec && dsum) out[n] += load_pack<T, VEC>(dsum + row * D + p);
     }
-    if (L > 64) __syncthreads();                       // dx may be dsum: packs that overlap at the row's end are read before they are written
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int i = lane + n * L;

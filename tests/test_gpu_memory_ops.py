@@ -177,6 +177,48 @@ def test_delta_rule_on_nothing(ops):
         assert (ops.gated_delta_rule(*[x.detach() for x in inputs])[1] == 0).all()
 
 
+@pytest.mark.parametrize("through", ["out", "state"])
+def test_delta_gradients_through_one_output_alone(ops, through):
+    g = gen(12)
+    inputs = delta_inputs(g, 2, 90, 2, 1, 20, 24, F32, 0.02)
+    leaves = [x.requires_grad_() for x in inputs] + [randn(g, 2, 2, 20, 24, scale=0.3).requires_grad_()]
+    wide = [x.detach().double().requires_grad_() for x in leaves]
+    i = 0 if through == "out" else 1
+    y, y64 = ops.gated_delta_rule(*leaves[:5], initial_state=leaves[5])[i], R.delta_rule(*wide[:5], wide[5])[i]
+    dy = randn(g, *y.shape)
+    got, want = torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y64, wide, dy.double(), allow_unused=True)
+    size = max((want[j] * wide[j]).detach().abs().sum(-1).max().item() for j in (0, 1) if want[j] is not None)
+    for j, (a, b) in enumerate(zip(got, want)):
+        b = torch.zeros_like(wide[j]) if b is None else torch.nan_to_num(b, nan=0.0)
+        R.close(a, b, 0, 4 * delta_terms(20, 24, 90), "gradient %d" % j, max(size, b.abs().max().item()) if j in (3, 4) else None)
+
+
+def test_time_major_block_as_documented(ops):
+    """The block over a time-major batch is the block over the turned one, and its output comes back time-major without a copy."""
+    g = gen(13)
+    T, rows, D, H, K, V = 70, 6, 48, 2, 16, 24
+    x, res, lengths = randn(g, T, rows, D), randn(g, T, rows, D), torch.tensor([70, 1, 0, 64, 33, 70], dtype=torch.int32, device="cuda")
+    nw, w, wo = 1 + randn(g, D, scale=0.1), randn(g, H * (2 * K + V), D, scale=D ** -0.5), randn(g, D, H * V, scale=0.1)
+    decay, beta = -0.1 * rand(g, T, rows, H), rand(g, T, rows, H)
+    turn = lambda t: t.transpose(0, 1)                                                   # noqa: E731
+
+    def block(x, res, decay, beta, major):
+        y, s = ops.rms_norm(x, nw, residual=res)
+        q, k, v = (t.unflatten(-1, (H, -1)) for t in ops.linear(y, w, activation="silu").split([H * K, H * K, H * V], -1))
+        k = torch.nn.functional.normalize(k, dim=-1)
+        o, S = ops.gated_delta_rule(*(turn(t) if major else t for t in (q, k, v, decay, beta)), lengths=lengths)
+        o = turn(o) if major else o
+        assert o.is_contiguous()
+        return ops.linear(o.flatten(-2), wo, residual=s), S
+    leaf = x.requires_grad_()
+    y, S = block(leaf, res, decay, beta, True)
+    leaf2 = turn(x.detach()).contiguous().requires_grad_()
+    y2, S2 = block(leaf2, turn(res).contiguous(), turn(decay).contiguous(), turn(beta).contiguous(), False)
+    assert torch.equal(turn(y), y2) and torch.equal(S, S2)
+    dy = randn(g, T, rows, D)
+    assert torch.equal(turn(torch.autograd.grad(y, leaf, dy)[0]), torch.autograd.grad(y2, leaf2, turn(dy))[0])
+
+
 def test_delta_gradient_agrees_with_differences(ops):
     g = gen(8)
     inputs = delta_inputs(g, 2, 100, 2, 1, 16, 12, F32) + [randn(g, 2, 2, 16, 12, scale=0.3)]
