@@ -104,6 +104,16 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   }
   return 1.f;
 }
+__device__ __forceinline__ f32x4 act4(f32x4 z, int act) {          // one branch for the four
+  const auto each = [&](auto a) { return f32x4{act_of(z[0], a()), act_of(z[1], a()), act_of(z[2], a()), act_of(z[3], a())}; };
+  switch (act) {
+    case OPE_ACT_RELU: return each(std::integral_constant<int, OPE_ACT_RELU>{});
+    case OPE_ACT_TANH: return each(std::integral_constant<int, OPE_ACT_TANH>{});
+    case OPE_ACT_SILU: return each(std::integral_constant<int, OPE_ACT_SILU>{});
+    case OPE_ACT_GELU: return each(std::integral_constant<int, OPE_ACT_GELU>{});
+  }
+  return z;
+}
 
 struct Epilogue {
   const float *x_scale, *w_scale;
@@ -135,9 +145,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, f32x4 acc, int64_t m,
   }
   if (e.x_scale) z *= sw * e.x_scale[m];
   z += b;
-  f32x4 y;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = act_of(z[r], e.act) + res[r];
+  const f32x4 y = act4(z, e.act) + res;
   const int64_t at = m * e.N + n;
   if (live == 4) {
     store_pack<O, 4>((O*)e.y + at, y);
@@ -158,11 +166,13 @@ struct Operand {
 };
 
 // One operand's tile of R output rows and 128 bytes of the contraction, on its way from memory through registers to LDS (TH threads). LDS rows are 8
-// pieces of 16 bytes, stored at piece ^ (row & 7) so that neither the stores nor the 16-row fragment reads collide in the banks.
+// pieces of 16 bytes, stored at piece ^ spread(row): 8 rows behind each other, and 8 rows 4 apart, then lie in 8 different places, so neither the
+// 16-row fragment reads nor the stores of turned columns collide in the banks.
 //   ALONG: the contraction runs along memory; a thread moves whole pieces.
 //   else: it runs over the rows of memory (gradients: dz^T x, dz w); a thread takes C neighbouring columns of as many rows as a piece has elements and
 //   turns them in registers, so nothing is transposed in memory. 16 neighbouring lanes read one run of a row, the four rows of lanes behind them
 //   other pieces: their LDS stores then spread over all eight places.
+__device__ __forceinline__ int spread(int row) { return (row ^ (row >> 2)) & 7; }
 template <typename T, int R, int TH, bool ALONG>
 struct Loader {
   static constexpr int N = R * 8 / TH;                                    // pieces a thread moves
@@ -228,13 +238,13 @@ struct Loader {
     if constexpr (ALONG) {
       const int row = threadIdx.x >> 3, piece = threadIdx.x & 7;
 #pragma unroll
-      for (int i = 0; i < N; ++i) lds[row + TH / 8 * i][piece ^ (row & 7)] = r[i];
+      for (int i = 0; i < N; ++i) lds[row + TH / 8 * i][piece ^ spread(row + TH / 8 * i)] = r[i];
     } else {
 #pragma unroll
       for (int i = 0; i < N / C; ++i) {
         const int x = threadIdx.x + TH * i, col = ((x & 15) + 16 * (x >> 7)) * C, piece = (x >> 4) & 7;
 #pragma unroll
-        for (int c = 0; c < C; ++c) lds[col + c][piece ^ ((col + c) & 7)] = r[C * i + c];
+        for (int c = 0; c < C; ++c) lds[col + c][piece ^ spread(col + c)] = r[C * i + c];
       }
     }
   }
@@ -286,9 +296,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B
     for (int h = 0; h < 2; ++h) {
       u32x4 fa[MT], fb[NT];
 #pragma unroll
-      for (int b = 0; b < NT; ++b) fb[b] = Bs[buf][wn + 16 * b + j][(4 * h + g) ^ (j & 7)];
+      for (int b = 0; b < NT; ++b) fb[b] = Bs[buf][wn + 16 * b + j][(4 * h + g) ^ spread(wn + 16 * b + j)];
 #pragma unroll
-      for (int a = 0; a < MT; ++a) fa[a] = As[buf][wm + 16 * a + j][(4 * h + g) ^ (j & 7)];
+      for (int a = 0; a < MT; ++a) fa[a] = As[buf][wm + 16 * a + j][(4 * h + g) ^ spread(wm + 16 * a + j)];
 #pragma unroll
       for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -322,16 +332,17 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B
   }
 }
 
-// Sums the splits and runs the epilogue: 16 packs of 4 outputs a workgroup, 16 runs of splits side by side and then in order.
-template <typename O>
+// Sums the splits in order and runs the epilogue: a pack of 4 outputs a thread; RUNS > 1 (many splits of a small output): 16 packs a workgroup, 16 runs
+// of splits side by side, then the runs in order. (8 splits and fewer leave half of the runs idle: 37 against 9 us for two splits of 2000 x 1500.)
+template <typename O, int RUNS>
 __global__ __launch_bounds__(256) void linear_join(const float* __restrict__ part, int splits, Epilogue e) {
-  __shared__ f32x4 lds[16][17];
-  const int per = ope_cdiv_dev4(e.N), run = threadIdx.x >> 4;
-  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), m = i / per;
+  constexpr int PACKS = 256 / RUNS;
+  const int per = ope_cdiv_dev4(e.N), run = threadIdx.x / PACKS;
+  const int64_t i = (int64_t)blockIdx.x * PACKS + (threadIdx.x % PACKS), m = i / per;
   const int n = (int)(i % per) * 4;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   if (m < e.M)
-    for (int s = run; s < splits; s += 16) {
+    for (int s = run; s < splits; s += RUNS) {
       const float* p = part + ((int64_t)s * e.M + m) * e.N + n;
       if (n + 4 <= e.N) acc += load_pack<float, 4>(p);
       else
@@ -339,11 +350,14 @@ __global__ __launch_bounds__(256) void linear_join(const float* __restrict__ par
         for (int r = 0; r < 4; ++r)
           if (n + r < e.N) acc[r] += p[r];
     }
-  lds[run][threadIdx.x & 15] = acc;
-  __syncthreads();
-  if (run) return;
-  acc = lds[0][threadIdx.x];
-  for (int r = 1; r < 16; ++r) acc += lds[r][threadIdx.x];
+  if constexpr (RUNS > 1) {
+    __shared__ f32x4 lds[RUNS][PACKS + 1];
+    lds[run][threadIdx.x % PACKS] = acc;
+    __syncthreads();
+    if (run) return;
+    acc = lds[0][threadIdx.x];
+    for (int r = 1; r < RUNS; ++r) acc += lds[r][threadIdx.x];
+  }
   finish4<O>(e, acc, m, n);
 }
 
@@ -403,43 +417,52 @@ __global__ __launch_bounds__(512) void linear_few(Operand A, Operand B, int64_t 
 }
 
 // dz = dy act'(z), and the column sums of dz over a workgroup's kDzRows rows for dbias. 64 columns a workgroup; 4 neighbouring columns a lane, 16 rows side
-// by side. Without an activation (z = NULL) only the sums.
-constexpr int kDzRows = 256;
-template <typename T>
-__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const float* __restrict__ z, int64_t M, int N, int act, T* __restrict__ dz,
+// by side, all of a thread's loads before their first use. Without an activation only the sums. A kernel for each activation: with the choice inside,
+// the code of all of them, unrolled, did not stay in the instruction cache (14 us for any small batch).
+constexpr int kDzRows = 128;
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const float* __restrict__ z, int64_t M, int N, T* __restrict__ dz,
                                                  float* __restrict__ sums) {
+  constexpr int R = kDzRows / 16;
   __shared__ f32x4 lds[16][17];
   const int tn = ope_cdiv_dev64(N), n = (int)(blockIdx.x % tn) * 64 + (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
   const int64_t m0 = (int64_t)(blockIdx.x / tn) * kDzRows;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (n < N)
-#pragma unroll 4
-    for (int r = r0; r < kDzRows; r += 16) {
-      const int64_t m = m0 + r, at = m * N + n;
-      if (m >= M) break;
-      f32x4 d = {0.f, 0.f, 0.f, 0.f}, x = d;
-      if (n + 4 <= N) {
-        d = load_pack<T, 4>(dy + at);
-        if (z) x = load_pack<float, 4>(z + at);
-      } else {
+  if (n + 4 <= N) {
+    f32x4 d[R], x[R];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (n + c < N) {
-            d[c] = (float)dy[at + c];
-            if (z) x[c] = z[at + c];
-          }
-      }
-      if (z) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) d[c] *= act_slope(x[c], act);
-        if (n + 4 <= N) store_pack<T, 4>(dz + at, d);
-        else
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (n + c < N) dz[at + c] = (T)d[c];
-      }
-      s += d;
+    for (int i = 0; i < R; ++i) {                       // (rows past the last one read the last one's values again)
+      const int64_t at = min(m0 + r0 + 16 * i, M - 1) * N + n;
+      d[i] = load_pack<T, 4>(dy + at);
+      if constexpr (ACT != OPE_ACT_NONE) x[i] = load_pack<float, 4>(z + at);
     }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t m = m0 + r0 + 16 * i;
+      if (m >= M) break;
+      if constexpr (ACT != OPE_ACT_NONE) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) d[i][c] *= act_slope(x[i][c], ACT);
+        store_pack<T, 4>(dz + m * N + n, d[i]);
+      }
+      s += d[i];
+    }
+  } else if (n < N) {
+    for (int i = 0; i < R; ++i) {
+      const int64_t m = m0 + r0 + 16 * i;
+      if (m >= M) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (n + c < N) {
+          float d = (float)dy[m * N + n + c];
+          if constexpr (ACT != OPE_ACT_NONE) {
+            d *= act_slope(z[m * N + n + c], ACT);
+            dz[m * N + n + c] = (T)d;
+          }
+          s[c] += d;
+        }
+    }
+  }
   if (!sums) return;
   lds[r0][threadIdx.x & 15] = s;
   __syncthreads();
@@ -467,22 +490,26 @@ __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ s
 }
 
 // How one product is cut: the tile, and splits of k where the tiles alone leave CUs idle. Short contractions (under 8 steps of 128 bytes) and
-// small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least: a
-// round of 256 x 256 tiles (one a CU) is 4 units of work, one of 128 x 128 tiles (two a CU) 2 units at about 0.8 of the rate.
+// small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least, in units
+// of a 64 x 64 tile's work a CU at the rates measured for each (0.55, 0.85 and 1 of the largest's).
 struct Cut { int BM, tm, tn, steps, splits, per; bool few; };
 static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few) {
   Cut c;
   c.few = may_be_few && M <= 64;
   c.steps = (int)((klen + 127) / 128);
-  const int64_t t128 = (int64_t)ope_cdiv(M, 128) * ope_cdiv(N, 128), t256 = (int64_t)ope_cdiv(M, 256) * ope_cdiv(N, 256);
   c.BM = 64;
-  if (M > 64 && N > 64 && t128 >= 256 && c.steps >= 8) c.BM = 4.0 * ((t256 + 255) / 256) < 2.5 * ((t128 + 511) / 512) ? 256 : 128;
+  if (M > 64 && N > 64 && c.steps >= 8 && (int64_t)ope_cdiv(M, 128) * ope_cdiv(N, 128) >= 256) {
+    auto rounds = [&](int t) { return (double)(((int64_t)ope_cdiv(M, t) * ope_cdiv(N, t) + 255) / 256); };
+    const double c64 = rounds(64) / 0.55, c128 = 4 * rounds(128) / 0.85, c256 = 16 * rounds(256);
+    if (c128 < c64) c.BM = 128;
+    if (c256 < c128 && c256 < c64) c.BM = 256;
+  }
   c.tm = ope_cdiv(M, c.BM);
   c.tn = ope_cdiv(N, c.BM);
   const int64_t tiles = (int64_t)c.tm * c.tn;
   c.splits = 1;
-  if (!c.few && tiles && tiles < 256) {        // (no rows: no tiles)
-    const int64_t want = 512 / tiles, most = c.steps / 4;      // two workgroups a CU, four steps at least each
+  if (!c.few && c.BM == 64 && tiles && tiles < 512) {          // (no rows: no tiles)
+    const int64_t want = 1024 / tiles, most = c.steps / 4;     // four workgroups a CU, four steps at least each
     c.splits = (int)(want < most ? want : most);
     if (c.splits < 1) c.splits = 1;
   }
@@ -513,7 +540,8 @@ static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e,
   OPE_CHECK_LAUNCH();
   if (c.splits > 1) {
     const int64_t n = e.M * ((e.N + 3) / 4);
-    OPE_LAUNCH((linear_join<O>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, c.splits, e);
+    if (c.splits > 8) OPE_LAUNCH((linear_join<O, 16>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, c.splits, e);
+    else OPE_LAUNCH((linear_join<O, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, c.splits, e);
     OPE_CHECK_LAUNCH();
   }
   return OPE_OK;
@@ -603,8 +631,16 @@ extern "C" int ope_linear_backward(const ope_linear_cfg* cfg, const void* dy, co
     const T* dz = acts ? (const T*)(ws + p.dz) : (const T*)dy;
     const int tm = ope_cdiv(M, kDzRows);
     if (acts || dbias) {
-      OPE_LAUNCH((linear_dz<T>), dim3((unsigned)((int64_t)tm * ope_cdiv(N, 64))), dim3(256), 0, st, (const T*)dy, acts ? z : nullptr, M, N, cfg->activation,
-                 acts ? (T*)(ws + p.dz) : nullptr, dbias ? (float*)(ws + p.sums) : nullptr);
+      const dim3 grid((unsigned)((int64_t)tm * ope_cdiv(N, 64)));
+      T* const out = acts ? (T*)(ws + p.dz) : nullptr;
+      float* const sums = dbias ? (float*)(ws + p.sums) : nullptr;
+      switch (cfg->activation) {
+        case OPE_ACT_NONE: OPE_LAUNCH((linear_dz<T, OPE_ACT_NONE>), grid, dim3(256), 0, st, (const T*)dy, z, M, N, out, sums); break;
+        case OPE_ACT_RELU: OPE_LAUNCH((linear_dz<T, OPE_ACT_RELU>), grid, dim3(256), 0, st, (const T*)dy, z, M, N, out, sums); break;
+        case OPE_ACT_TANH: OPE_LAUNCH((linear_dz<T, OPE_ACT_TANH>), grid, dim3(256), 0, st, (const T*)dy, z, M, N, out, sums); break;
+        case OPE_ACT_SILU: OPE_LAUNCH((linear_dz<T, OPE_ACT_SILU>), grid, dim3(256), 0, st, (const T*)dy, z, M, N, out, sums); break;
+        case OPE_ACT_GELU: OPE_LAUNCH((linear_dz<T, OPE_ACT_GELU>), grid, dim3(256), 0, st, (const T*)dy, z, M, N, out, sums); break;
+      }
       OPE_CHECK_LAUNCH();
     }
     if (dbias) {
