@@ -493,7 +493,7 @@ __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ s
 // small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least, in units
 // of a 64 x 64 tile's work a CU at the rates measured for each (0.55, 0.85 and 1 of the largest's).
 struct Cut { int BM, tm, tn, steps, splits, per; bool few; };
-static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few) {
+static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few, int eb) {
   Cut c;
   c.few = may_be_few && M <= 64;
   c.steps = (int)((klen + 127) / 128);
@@ -513,6 +513,9 @@ static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few) {
     c.splits = (int)(want < most ? want : most);
     if (c.splits < 1) c.splits = 1;
   }
+  // One 128 x 128 tile a CU leaves it idle at every barrier; in float32 a second split pays for its join (dw of 4096 x 2048 x 2048: 393 against 293 + 9
+  // us), in 16 bits the join's bytes would cost as much as the product gains.
+  if (c.BM == 128 && eb == 4 && tiles < 512 && c.steps >= 32) c.splits = 2;
   c.per = ope_cdiv(c.steps, c.splits);
   if (c.per < 1) c.per = 1;
   c.splits = c.steps ? ope_cdiv(c.steps, c.per) : 1;
@@ -523,7 +526,7 @@ static int64_t cut_floats(const Cut& c, int64_t M, int64_t N) { return c.splits 
 // AA, BA: the contraction runs along memory in A / B
 template <typename T, typename O, bool AA, bool BA>
 static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e, float* part, hipStream_t st) {
-  const Cut c = cut_of(e.M, e.N, klen, AA && BA);
+  const Cut c = cut_of(e.M, e.N, klen, AA && BA, (int)sizeof(T));
   if constexpr (AA && BA)
     if (c.few) {
       const dim3 grid((unsigned)ope_cdiv(e.N, 16));
@@ -565,8 +568,8 @@ static BwdPlan bwd_plan(const ope_linear_cfg* c) {
   auto take = [&](int64_t bytes) { const int64_t r = o; o += (bytes + 255) & ~(int64_t)255; return r; };
   p.dz = take(c->activation != OPE_ACT_NONE ? M * N * eb : 0);
   p.sums = take((int64_t)ope_cdiv(M, kDzRows) * N * 4);
-  p.part_dx = take(cut_floats(cut_of(M, K, N * eb, false), M, K) * 4);
-  p.part_dw = take(cut_floats(cut_of(N, K, M * eb, false), N, K) * 4);
+  p.part_dx = take(cut_floats(cut_of(M, K, N * eb, false, (int)eb), M, K) * 4);
+  p.part_dw = take(cut_floats(cut_of(N, K, M * eb, false, (int)eb), N, K) * 4);
   p.bytes = o;
   return p;
 }
@@ -582,7 +585,7 @@ using namespace ope;
 
 extern "C" int64_t ope_linear_workspace_bytes(const ope_linear_cfg* cfg) {
   if (!linear_ok(cfg)) return OPE_EINVAL;
-  return cut_floats(cut_of(cfg->rows, cfg->out_width, (int64_t)cfg->in_width * elem_bytes(cfg->dtype), true), cfg->rows, cfg->out_width) * 4;
+  return cut_floats(cut_of(cfg->rows, cfg->out_width, (int64_t)cfg->in_width * elem_bytes(cfg->dtype), true, elem_bytes(cfg->dtype)), cfg->rows, cfg->out_width) * 4;
 }
 
 extern "C" int ope_linear(const ope_linear_cfg* cfg, const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,

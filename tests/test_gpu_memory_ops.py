@@ -486,6 +486,13 @@ def test_linear_wide_tiles(ops):
         check_linear(ops, g, M, K, N, dtype, "none", True, False)
 
 
+def test_linear_wide_outputs_whose_contraction_is_split(ops):
+    """Two splits of float32 tiles of 128 (forward), and of tiles of 64 (gradients), in odd sizes, joined with the whole epilogue."""
+    g = gen(41)
+    check_linear(ops, g, 2100, 1030, 2050, F32, "gelu")
+    check_linear(ops, g, 1203, 1101, 1003, BF16, "tanh")
+
+
 def test_linear_takes_rows_of_any_stride_and_no_rows(ops):
     g = gen(34)
     wide = randn(g, 90, 301, dtype=BF16)
