@@ -145,7 +145,7 @@ def _pack_step(plan, scale, q, k, v, g, beta):
 
 def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
     """One token of gated_delta_rule for every row: q, k [B, Hk, K], v [B, H, V], log_decay, beta float32 [B, H]; `state` float32 [B, H, K, V], contiguous,
-    is updated in place (log_decay = -inf: cleared first, whatever it holds). Returns out [B, H, V]. For acting: no gradients."""
+    is updated in place and shares no memory with the other arguments (log_decay = -inf: cleared first, whatever it holds). Returns out [B, H, V]. For acting: no gradients."""
     tensors((state, "the state"))
     plan = _check(q, k, v, log_decay, beta, state, None, 1)
     if not state.is_contiguous():
@@ -159,4 +159,5 @@ def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
                        log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), stream())
         if rc:
             _lib.check(rc, "ope_delta_step")
+    torch._C._increment_version((state,))          # a graph that holds the old state refuses to go on with the new one
     return o

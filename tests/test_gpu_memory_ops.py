@@ -663,6 +663,20 @@ def test_captured_training_pass_replays(ops):
                 assert torch.equal(a, b)
 
 
+def test_a_step_is_seen_by_graphs_that_hold_the_state(ops):
+    """The step changes the state in place: as after any in-place change, a graph that saved it refuses its backward pass."""
+    g = gen(47)
+    args = [x[:, 0].contiguous() for x in delta_inputs(g, 4, 1, 2, 2, 32, 32, F32)]
+    state, w = randn(g, 4, 2, 32, 32), randn(g, 4, 2, 32, 32).requires_grad_()
+    loss = (state * w).sum()
+    with torch.no_grad():
+        ops.gated_delta_step(*args, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        ops.gated_delta_step(*args, state.clone())
+
+
 def test_captured_step_replays(ops):
     g = gen(43)
     args = [x[:, 0].contiguous() for x in delta_inputs(g, 8, 1, 2, 2, 32, 32, F32)]
