@@ -128,7 +128,7 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
 def linear_fp8(x, x_scale, weight, w_scale, bias=None, residual=None, activation="none", out_dtype=torch.bfloat16):
     """y = act((x weight^T) x_scale w_scale + bias) + residual with 8-bit operands, as rms_norm_fp8 and quantize_rows_fp8 return them: x [..., in]
     and weight [out, in] float8_e4m3fn, x_scale float32 of x.shape[:-1], w_scale float32 [out]; bias and residual of out_dtype. For acting: no gradients
-    (a scale, bias or residual that requires one is refused while gradients are recorded)."""
+    (an argument that requires one is refused while gradients are recorded)."""
     tensors((x, "x"), (x_scale, "x_scale"), (w_scale, "w_scale"))
     same_dtype(x.dtype, "x", E4M3)
     plan = _check(x, weight, bias, residual, activation, out_dtype)
@@ -136,7 +136,7 @@ def linear_fp8(x, x_scale, weight, w_scale, bias=None, residual=None, activation
         raise ValueError("x_scale and w_scale: shapes %s and %s wanted, got %s and %s" % (tuple(x.shape[:-1]), tuple(weight.shape[:1]), tuple(x_scale.shape), tuple(w_scale.shape)))
     same_dtype(x_scale.dtype, "x_scale", torch.float32)
     same_dtype(w_scale.dtype, "w_scale", torch.float32)
-    if wants_grad(x_scale, w_scale, bias, residual):
+    if wants_grad(x, x_scale, weight, w_scale, bias, residual):
         raise ValueError("linear_fp8 has no gradients: call it under torch.no_grad(), or linear")
     with on_device(x, x_scale, weight, w_scale, bias, residual):
         return _forward(plan, x, weight, x_scale.contiguous(), w_scale.contiguous(), bias, residual, out_dtype, False)[0]

@@ -88,6 +88,16 @@ def test_linear_refuses():
             ops.linear_fp8(*a, **more)
 
 
+def test_acting_forms_refuse_arguments_that_want_gradients():
+    x8, w8, xs, ws = torch.zeros(3, 8).to(E4M3), torch.zeros(5, 8).to(E4M3), torch.ones(3), torch.ones(5)
+    for i in range(4):
+        a = [t.clone().requires_grad_(i == j) for j, t in enumerate((x8, xs, w8, ws))]
+        with pytest.raises(ValueError, match="no gradients"):
+            ops.linear_fp8(*a)
+    with pytest.raises(ValueError, match="no gradients"):
+        ops.quantize_rows_fp8(torch.zeros(3, 8, requires_grad=True))
+
+
 def test_there_is_no_cpu_path():
     with pytest.raises(ValueError, match="GPU only"):
         ops.gated_delta_rule(*delta_args())
