@@ -35,7 +35,7 @@ static inline DeltaDims delta_dims(const ope_delta_cfg* c) {
   DeltaDims d;
   d.B = c->batch; d.T = c->seq_len; d.H = c->n_heads; d.Hk = c->n_qk_heads; d.K = c->key_dim; d.V = c->value_dim;
   d.n = ope_cdiv(d.T, kC);
-  d.KT = d.K <= 16 ? 1 : d.K <= 32 ? 2 : d.K <= 64 ? 4 : 8;
+  d.KT = d.K <= 16 ? 1 : d.K <= 32 ? 2 : d.K <= 48 ? 3 : d.K <= 64 ? 4 : d.K <= 96 ? 6 : 8;
   d.VT = ope_cdiv(d.V, 16);
   d.Kp = 16 * d.KT; d.Vp = 16 * d.VT;
   d.chunks = (int64_t)d.B * d.H * d.n;

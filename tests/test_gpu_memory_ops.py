@@ -90,6 +90,13 @@ DELTA = [
     (2, 200, 2, 2, 64, 40, F32, 0, True),
     (5, 150, 2, 2, 32, 32, F32, 0.03, True),
     (1, 129, 1, 1, 127, 257, F16, 0, False),
+    (2, 140, 2, 1, 33, 20, F32, 0.03, False),
+    (3, 131, 2, 2, 48, 48, BF16, 0, True),
+    (2, 190, 4, 2, 48, 17, F16, 0, False),
+    (2, 260, 2, 2, 96, 96, F32, 0.02, False),
+    (1, 130, 2, 1, 96, 64, F16, 0, True),
+    (2, 70, 2, 2, 65, 130, BF16, 0, False),
+    (1, 200, 1, 1, 97, 30, F32, 0, False),
 ]
 
 
