@@ -1,7 +1,7 @@
 // Shared pieces of the gated delta rule's kernels (ope_delta.hip: forward and one-token step; ope_delta_bwd.hip: gradients).
 //
 // Names: a CHUNK is 64 tokens of one (sequence, head) = "chunk-head" c = (b * H + h) * n + i. Kp / Vp are the key and value widths padded to the
-// tiles of 16 the kernels work in (Kp to 16, 32, 64 or 128). Arithmetic is float32 throughout, on the f32 matrix instruction of ope_common.h:
+// tiles of 16 the kernels work in (Kp: 16 to 96, or 128). Arithmetic is float32 throughout, on the f32 matrix instruction of ope_common.h:
 // its "transposed chain" (lane (j, g) holds features 4g .. 4g+3 of data row j) is both the form a product leaves and the form the next one
 // reads, so the triangular solve and the scan need no shuffles.
 //
@@ -35,7 +35,7 @@ static inline DeltaDims delta_dims(const ope_delta_cfg* c) {
   DeltaDims d;
   d.B = c->batch; d.T = c->seq_len; d.H = c->n_heads; d.Hk = c->n_qk_heads; d.K = c->key_dim; d.V = c->value_dim;
   d.n = ope_cdiv(d.T, kC);
-  d.KT = d.K <= 16 ? 1 : d.K <= 32 ? 2 : d.K <= 48 ? 3 : d.K <= 64 ? 4 : d.K <= 96 ? 6 : 8;
+  d.KT = d.K > 96 ? 8 : ope_cdiv(d.K, 16);            // (seven tiles spill more registers of the backward pass than eight)
   d.VT = ope_cdiv(d.V, 16);
   d.Kp = 16 * d.KT; d.Vp = 16 * d.VT;
   d.chunks = (int64_t)d.B * d.H * d.n;

@@ -385,7 +385,7 @@ int launch_delta_scan(int dtype, const DeltaDims& d, bool bwd, const int32_t* le
     if (bwd) OPE_LAUNCH((delta_scan<T, KT, true>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, tails, first, last);     \
     else OPE_LAUNCH((delta_scan<T, KT, false>), grid, dim3(256), 0, st, d, lengths, M1, M2, UT, ST, gC, tails, first, last);        \
     break
-    switch (d.KT) { OPE_SCAN(1); OPE_SCAN(2); OPE_SCAN(3); OPE_SCAN(4); OPE_SCAN(6); OPE_SCAN(8); }
+    switch (d.KT) { OPE_SCAN(1); OPE_SCAN(2); OPE_SCAN(3); OPE_SCAN(4); OPE_SCAN(5); OPE_SCAN(6); OPE_SCAN(8); }
 #undef OPE_SCAN
     OPE_CHECK_LAUNCH();
     return OPE_OK;
@@ -444,14 +444,14 @@ extern "C" int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const 
     const dim3 grid((unsigned)d.chunks);
 #define OPE_PREP(KT) \
   case KT: OPE_LAUNCH((delta_prep<T, KT>), grid, dim3(64 * chunk_waves<KT>()), 0, st, *cfg, d, (const T*)k, (const T*)v, g, beta, lengths, W, WT, (T*)KTs, UT, gC, tails); break
-    switch (d.KT) { OPE_PREP(1); OPE_PREP(2); OPE_PREP(3); OPE_PREP(4); OPE_PREP(6); OPE_PREP(8); }
+    switch (d.KT) { OPE_PREP(1); OPE_PREP(2); OPE_PREP(3); OPE_PREP(4); OPE_PREP(5); OPE_PREP(6); OPE_PREP(8); }
 #undef OPE_PREP
     OPE_CHECK_LAUNCH();
     const int rc = launch_delta_scan(cfg->dtype, d, false, lengths, W, KTs, UT, ST, gC, tails, state0, state_out, st);
     if (rc) return rc;
 #define OPE_OUT(KT) \
   case KT: OPE_LAUNCH((delta_out<T, KT>), grid, dim3(256), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, ST, UT, (T*)o); break
-    switch (d.KT) { OPE_OUT(1); OPE_OUT(2); OPE_OUT(3); OPE_OUT(4); OPE_OUT(6); OPE_OUT(8); }
+    switch (d.KT) { OPE_OUT(1); OPE_OUT(2); OPE_OUT(3); OPE_OUT(4); OPE_OUT(5); OPE_OUT(6); OPE_OUT(8); }
 #undef OPE_OUT
     OPE_CHECK_LAUNCH();
     return OPE_OK;

@@ -25,7 +25,7 @@ template <typename T, int KT>
 __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta_bwd_prep(
     ope_delta_cfg cfg, DeltaDims d, const T* __restrict__ q_in, const T* __restrict__ k_in, const float* __restrict__ g_in, const float* __restrict__ beta_in,
     const int32_t* __restrict__ lengths, const T* __restrict__ dO, T* __restrict__ Ks, float* __restrict__ dUT, float* __restrict__ dST) {
-  constexpr int NW = chunk_waves<KT>(), RS = Rows<T, KT>::kStride;
+  constexpr int NW = chunk_waves<KT>(), RS = Rows<T, KT>::kStride, kPair = KT % 2 ? 1 : 2;
   __shared__ Rows<T, KT> q, k;
   __shared__ float PT[kC][kC + 4];
   __shared__ Gates gt;
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.head[16 * it + 4 * g]) * cfg.scale;
-#pragma unroll 2
+#pragma unroll kPair                                     // (all of an odd number of tiles would be unrolled, into scratch memory)
     for (int kt = 0; kt < KT; ++kt) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -380,7 +380,7 @@ extern "C" int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const
     const dim3 grid((unsigned)d.chunks);
 #define OPE_BPREP(KT) \
   case KT: OPE_LAUNCH((delta_bwd_prep<T, KT>), grid, dim3(64 * chunk_waves<KT>()), 0, st, *cfg, d, (const T*)q, (const T*)k, g, beta, lengths, (const T*)d_o, (T*)Ks, dUT, dST); break
-    switch (d.KT) { OPE_BPREP(1); OPE_BPREP(2); OPE_BPREP(3); OPE_BPREP(4); OPE_BPREP(6); OPE_BPREP(8); }
+    switch (d.KT) { OPE_BPREP(1); OPE_BPREP(2); OPE_BPREP(3); OPE_BPREP(4); OPE_BPREP(5); OPE_BPREP(6); OPE_BPREP(8); }
 #undef OPE_BPREP
     OPE_CHECK_LAUNCH();
     const int rc = launch_delta_scan(cfg->dtype, d, true, lengths, Ks, WT, dUT, dST, gC, tails, d_state, d_state0, st);
@@ -388,7 +388,7 @@ extern "C" int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const
 #define OPE_BMAIN(KT)                                                                                                                                  \
   case KT: OPE_LAUNCH((delta_bwd_main<T, KT>), grid, dim3(512), 0, st, *cfg, d, (const T*)q, (const T*)k, (const T*)v, g, beta, lengths, ST, UT,        \
                       (const T*)d_o, dUT, dST, (T*)dq, (T*)dk, dqp, dkp, (T*)dv, dg, dbeta); break
-    switch (d.KT) { OPE_BMAIN(1); OPE_BMAIN(2); OPE_BMAIN(3); OPE_BMAIN(4); OPE_BMAIN(6); OPE_BMAIN(8); }
+    switch (d.KT) { OPE_BMAIN(1); OPE_BMAIN(2); OPE_BMAIN(3); OPE_BMAIN(4); OPE_BMAIN(5); OPE_BMAIN(6); OPE_BMAIN(8); }
 #undef OPE_BMAIN
     OPE_CHECK_LAUNCH();
     if (d.H != d.Hk) {

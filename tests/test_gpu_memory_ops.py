@@ -97,6 +97,9 @@ DELTA = [
     (1, 130, 2, 1, 96, 64, F16, 0, True),
     (2, 70, 2, 2, 65, 130, BF16, 0, False),
     (1, 200, 1, 1, 97, 30, F32, 0, False),
+    (2, 150, 2, 1, 80, 36, F32, 0.02, True),
+    (1, 260, 2, 2, 112, 112, BF16, 0, False),
+    (2, 129, 2, 2, 103, 20, F32, 0, False),
 ]
 
 
