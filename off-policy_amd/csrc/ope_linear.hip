@@ -333,7 +333,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B
 }
 
 // Sums the splits in order and runs the epilogue: a pack of 4 outputs a thread; RUNS > 1 (many splits of a small output): 16 packs a workgroup, 16 runs
-// of splits side by side, then the runs in order. (8 splits and fewer leave half of the runs idle: 37 against 9 us for two splits of 2000 x 1500.)
+// of splits side by side, then the runs in order. (8 splits and fewer leave half of the runs idle: two of 2000 x 1500 took 37 us
+// that way; a pack a thread takes 9 for two of 2048 x 2048.)
 template <typename O, int RUNS>
 __global__ __launch_bounds__(256) void linear_join(const float* __restrict__ part, int splits, Epilogue e) {
   constexpr int PACKS = 256 / RUNS;
@@ -490,8 +491,11 @@ __global__ __launch_bounds__(1024) void linear_dbias(const float* __restrict__ s
 }
 
 // How one product is cut: the tile, and splits of k where the tiles alone leave CUs idle. Short contractions (under 8 steps of 128 bytes) and
-// small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least, in units
-// of a 64 x 64 tile's work a CU at the rates measured for each (0.55, 0.85 and 1 of the largest's).
+// small outputs are bound by memory and latency: tiles of 64 x 64, five workgroups a CU. Otherwise the tile whose rounds over the chip cost least, in
+// the time of a 64 x 64 tile's work at the rates measured for each:
+//   bf16, 4096 x 4096 x 4096 : 588 / 816 / 973 TFLOP/s with tiles of 64 / 128 / 256; a tile of 128 that is alone on its CU waits for itself at every
+//                              barrier (2048 x 2048 x 2048, one tile a CU: 493 against 527 with tiles of 64);
+//   float32                  : 114 / 132 / 112.
 struct Cut { int BM, tm, tn, steps, splits, per; bool few; };
 static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few, int eb) {
   Cut c;
@@ -499,10 +503,15 @@ static Cut cut_of(int64_t M, int64_t N, int64_t klen, bool may_be_few, int eb) {
   c.steps = (int)((klen + 127) / 128);
   c.BM = 64;
   if (M > 64 && N > 64 && c.steps >= 8 && (int64_t)ope_cdiv(M, 128) * ope_cdiv(N, 128) >= 256) {
-    auto rounds = [&](int t) { return (double)(((int64_t)ope_cdiv(M, t) * ope_cdiv(N, t) + 255) / 256); };
-    const double c64 = rounds(64) / 0.55, c128 = 4 * rounds(128) / 0.85, c256 = 16 * rounds(256);
-    if (c128 < c64) c.BM = 128;
-    if (c256 < c128 && c256 < c64) c.BM = 256;
+    auto rounds = [&](int t) { return ((int64_t)ope_cdiv(M, t) * ope_cdiv(N, t) + 255) / 256; };
+    const int64_t n = rounds(128);
+    if (eb == 4) {
+      if (4 * n < rounds(64) / 0.86) c.BM = 128;
+    } else {
+      const double c64 = rounds(64) / 0.6, c128 = 4 * ((n - n % 2) / 0.83 + n % 2 / 0.55), c256 = 16. * rounds(256);
+      if (c128 < c64) c.BM = 128;
+      if (c256 < c128 && c256 < c64) c.BM = 256;
+    }
   }
   c.tm = ope_cdiv(M, c.BM);
   c.tn = ope_cdiv(N, c.BM);
@@ -537,9 +546,9 @@ static int launch_product(Operand A, Operand B, int64_t klen, const Epilogue& e,
       return OPE_OK;
     }
   const dim3 grid((unsigned)((int64_t)c.tm * c.tn), (unsigned)c.splits);
-  if (c.BM == 256) OPE_LAUNCH((linear_tile<T, O, 256, 256, 2, 4, AA, BA>), grid, dim3(512), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
+  if (c.BM == 64) OPE_LAUNCH((linear_tile<T, O, 64, 64, 2, 2, AA, BA>), grid, dim3(256), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
   else if (c.BM == 128) OPE_LAUNCH((linear_tile<T, O, 128, 128, 2, 2, AA, BA>), grid, dim3(256), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
-  else OPE_LAUNCH((linear_tile<T, O, 64, 64, 2, 2, AA, BA>), grid, dim3(256), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
+  else if constexpr (sizeof(T) < 4) OPE_LAUNCH((linear_tile<T, O, 256, 256, 2, 4, AA, BA>), grid, dim3(512), 0, st, A, B, klen, c.tm, c.tn, c.per, e, part);
   OPE_CHECK_LAUNCH();
   if (c.splits > 1) {
     const int64_t n = e.M * ((e.N + 3) / 4);

@@ -500,7 +500,14 @@ def test_linear_wide_outputs_whose_contraction_is_split(ops):
     """Two splits of float32 tiles of 128 (forward), and of tiles of 64 (gradients), in odd sizes, joined with the whole epilogue."""
     g = gen(41)
     check_linear(ops, g, 2100, 1030, 2050, F32, "gelu")
+    check_linear(ops, g, 2040, 1030, 2045, F32, "gelu")
     check_linear(ops, g, 1203, 1101, 1003, BF16, "tanh")
+
+
+@pytest.mark.parametrize("M,K,N,dtype", [(4090, 300, 2045, F32), (4090, 600, 2045, BF16), (4090, 520, 4090, F16)])
+def test_linear_tiles_of_every_size(ops, M, K, N, dtype):
+    """The tiles of 128 (float32, 16 bits) and of 256 in odd sizes, with the whole epilogue."""
+    check_linear(ops, gen(48), M, K, N, dtype, "silu")
 
 
 def test_linear_takes_rows_of_any_stride_and_no_rows(ops):
