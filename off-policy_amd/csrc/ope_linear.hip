@@ -82,6 +82,19 @@ __device__ __forceinline__ u32x4 row16(const uint8_t* row, int64_t k, int64_t le
   }
   return v;
 }
+// The last step of float32 rows that end inside it, for the forward product: piece g of a half (16 values) takes k = 4 r + g, so that the matrix
+// instructions add what is left in ascending order of k. Whole steps go by k = 4 g + r (16 bytes a lane); with both, z is to the bit what the library's
+// float32 product of the same row gives where neither splits k, and a relu's gate falls on the same side where z is within rounding of 0 (one that falls
+// otherwise moves a row of dx and a row of dw). The loads are single ones there anyway.
+__device__ __forceinline__ u32x4 last16(const uint8_t* row, int64_t half, int g, int64_t len) {
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t k = half + 16 * r + 4 * g;
+    if (k < len) v[r] = *reinterpret_cast<const uint32_t*>(row + k);
+  }
+  return v;
+}
 
 // 1 / (1 + e^-z) by the hardware's 2^x and 1/x, each within one step of float32: with expf and a division the epilogue of a 4096 x 4096 output took
 // 20 us more than without an activation. e^-z past the range is infinite, its reciprocal 0.
@@ -168,12 +181,12 @@ struct Operand {
 // One operand's tile of R output rows and 128 bytes of the contraction, on its way from memory through registers to LDS (TH threads). LDS rows are 8
 // pieces of 16 bytes, stored at piece ^ spread(row): 8 rows behind each other, and 8 rows 4 apart, then lie in 8 different places, so neither the
 // 16-row fragment reads nor the stores of turned columns collide in the banks.
-//   ALONG: the contraction runs along memory; a thread moves whole pieces.
+//   ALONG: the contraction runs along memory; a thread moves whole pieces. LAST: by last16 in the step that the rows end in.
 //   else: it runs over the rows of memory (gradients: dz^T x, dz w); a thread takes C neighbouring columns of as many rows as a piece has elements and
 //   turns them in registers, so nothing is transposed in memory. 16 neighbouring lanes read one run of a row, the four rows of lanes behind them
 //   other pieces: their LDS stores then spread over all eight places.
 __device__ __forceinline__ int spread(int row) { return (row ^ (row >> 2)) & 7; }
-template <typename T, int R, int TH, bool ALONG>
+template <typename T, int R, int TH, bool ALONG, bool LAST>
 struct Loader {
   static constexpr int N = R * 8 / TH;                                    // pieces a thread moves
   static constexpr int E = 16 / (int)sizeof(T), C = N < 4 ? N : 4;        // elements of a piece; columns a thread takes
@@ -190,7 +203,9 @@ struct Loader {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const uint8_t* p = o.p + min(first + row + TH / 8 * i, o.rows - 1) * o.stride;
-        r[i] = WHOLE ? *reinterpret_cast<const u32x4_loose*>(p + k) : row16(p, k, klen, (int)sizeof(T));
+        if (WHOLE) r[i] = *reinterpret_cast<const u32x4_loose*>(p + k);
+        else if (LAST) r[i] = last16(p, k & ~(int64_t)63, threadIdx.x & 3, klen);
+        else r[i] = row16(p, k, klen, (int)sizeof(T));
       }
     } else {
       typedef uint32_t words __attribute__((ext_vector_type(W)));
@@ -268,8 +283,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(Operand A, Operand B
   const int64_t m0 = (int64_t)(4 * band + in % high) * BM, n0 = (int64_t)(in / high) * BN;
   const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
   const int steps = (int)((klen + 127) / 128), first = blockIdx.y * steps_per, last = min(first + steps_per, steps);
-  Loader<T, BM, TH, AA> la;
-  Loader<T, BN, TH, BA> lb;
+  constexpr bool kLast = AA && BA && sizeof(T) == 4;   // (both operands alike)
+  Loader<T, BM, TH, AA, kLast> la;
+  Loader<T, BN, TH, BA, kLast> lb;
   const int whole = (int)(klen / 128);                 // steps without an end in them
   auto fetch = [&](int s) {
     if (s < whole) {

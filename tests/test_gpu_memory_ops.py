@@ -510,6 +510,31 @@ def test_linear_tiles_of_every_size(ops, M, K, N, dtype):
     check_linear(ops, gen(48), M, K, N, dtype, "silu")
 
 
+def in_order(x, w, order):
+    """x w^T in float32, one fused multiply-add for each k of `order` (a product of two float32 values is exact in 64 bits)."""
+    acc = torch.zeros(x.shape[0], w.shape[0], device="cuda")
+    for k in order:
+        acc = (acc.double() + x.double()[:, k, None] * w.double()[None, :, k]).float()
+    return acc
+
+
+@pytest.mark.parametrize("M,K,N", [(200, 30, 70), (200, 125, 70), (200, 128, 70), (32768, 252, 64)])
+def test_linear_float32_adds_up_in_the_stated_order(ops, M, K, N):
+    """Whole steps of 32 values by k = 16 s + 4 g + r (g innermost), what is left of the row in ascending order: a relu's gate at z = 0 hangs on it."""
+    g = gen(50)
+    x, w = randn(g, M, K), randn(g, N, K, scale=K ** -0.5)
+    whole = K // 32 * 32
+    order = [s + 4 * q + r for s in range(0, whole, 16) for r in range(4) for q in range(4)] + list(range(whole, K))
+    want = in_order(x[:96], w, order)
+    y = ops.linear(x, w)
+    assert torch.equal(y[:96], want)
+    leaf = x.detach().requires_grad_()
+    z = ops.linear(leaf, w, activation="relu")
+    assert torch.equal(z[:96], want.clamp_min(0))
+    dx = torch.autograd.grad(z, leaf, torch.ones_like(z))[0][:96]
+    R.close(dx, (want > 0).double() @ w.double(), 0, N + 2, "dx", w.abs().sum(0).max().item())
+
+
 def test_linear_takes_rows_of_any_stride_and_no_rows(ops):
     g = gen(34)
     wide = randn(g, 90, 301, dtype=BF16)
