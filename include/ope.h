@@ -731,7 +731,8 @@ int ope_quantize_rows(const ope_norm_cfg* cfg, const void* x, void* q, float* sc
  *         three with the strides given (in elements; a time-major batch is the same call with two strides exchanged). n_heads is a multiple
  *         of n_qk_heads: query / key head i serves the value heads [i * r, (i + 1) * r), r = n_heads / n_qk_heads.
  *   g     float32, log of the decay, beta float32: [batch][seq_len][n_heads], strides g_stride / beta_stride.
- *         g = -inf clears the state in front of the token (an episode boundary inside a row).
+ *         Where e^g is 0 in float32 (-inf, the type's lowest value, anything under -103.97) the state is cleared in front of the token (an
+ *         episode boundary inside a row).
  *   lengths  int32 [batch] or NULL: tokens t >= lengths[b] (clamped to [0, seq_len]) are neither read nor do anything; their o is 0.
  *   state0   float32 [batch][n_heads][key_dim][value_dim] or NULL (zeros); state_out the same shape: the state behind the last live token.
  * The forward pass works on chunks of 64 tokens: with G the running sum of g inside a chunk, A_ij = beta_i exp(G_i - G_j) k_i.k_j (i > j),
@@ -752,7 +753,7 @@ int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const void* k, co
 /* Gradients from d_o (of `dtype`, shape of o, strides o_stride) and d_state (float32, gradient of state_out; NULL = zeros): dq, dk (shape of q),
  * dv (shape of v) of `dtype`, dg, dbeta float32, with the strides dq_stride .. dbeta_stride (last axis contiguous), d_state0 float32 or NULL.
  * `saved` and the inputs are those of the forward call. Gradients of shared query / key heads are summed over their value heads in a fixed
- * order. dg is 0 where g = -inf; everything is 0 behind a row's length. */
+ * order. dg is 0 where e^g is; everything is 0 behind a row's length. */
 int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta,
                        const int32_t* lengths, const void* saved, int64_t saved_bytes, const void* d_o, const float* d_state, void* dq,
                        void* dk, void* dv, float* dg, float* dbeta, float* d_state0, void* workspace, int64_t workspace_bytes, void* stream);

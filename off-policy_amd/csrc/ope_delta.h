@@ -63,7 +63,8 @@ __device__ __forceinline__ ChunkAt chunk_at(const DeltaDims& d, const int32_t* l
 }
 
 // The chunk's gates in LDS. G is the running sum of g inside a segment of the chunk, as a pair of floats (hi + lo: differences of long sums
-// keep their last bits); a reset (g = -inf) starts a new segment with G = 0, and decays across segments are exactly 0: what lies behind a reset
+// keep their last bits); a reset (e^g = 0 in float32: -inf, and every g under -103.97, so that no finite stand-in for -inf swallows the small gates
+// that are added behind it) starts a new segment with G = 0, and decays across segments are exactly 0: what lies behind a reset
 // does not depend on what lies in front of it, to the last bit.
 struct Gates {
   float hi[kC], lo[kC], beta[kC], head[kC], tail[kC];   // head: decay from the chunk's start through t; tail: from t to its end
@@ -79,7 +80,7 @@ __device__ __forceinline__ void load_gates(Gates& s, const ope_delta_cfg& c, con
   const bool on = t < a.nv;
   const float gt = on ? g[a.b * c.g_stride[0] + (int64_t)(a.t0 + t) * c.g_stride[1] + a.h * c.g_stride[2]] : 0.f;
   const float bt = on ? beta[a.b * c.beta_stride[0] + (int64_t)(a.t0 + t) * c.beta_stride[1] + a.h * c.beta_stride[2]] : 0.f;
-  const bool cut = gt == -INFINITY;
+  const bool cut = expf(gt) == 0.f;                     // as the one-token step decides it
   const unsigned long long cuts = __ballot(cut);
   const int seg = __popcll(cuts & (~0ull >> (63 - t)));
   double G = cut ? 0.0 : (double)gt;

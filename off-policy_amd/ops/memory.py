@@ -117,12 +117,12 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
 
     q, k [B, T, Hk, K], v [B, T, H, V] of one type (float32, bfloat16, float16), any strides with a contiguous last axis (a time-major batch is
     passed as x.transpose(0, 1)); H is a multiple of Hk and value head h reads query / key head h // (H // Hk). K up to 128, V up to 1024.
-    log_decay, beta float32 [B, T, H]: log_decay is at most 0 in use; -inf clears the (finite) state in front of its token, as where a row of the
-    batch goes on with another episode. initial_state float32 [B, H, K, V] (None: zeros). lengths int32 [B] (None: T): tokens at and behind
+    log_decay, beta float32 [B, T, H]: log_decay is at most 0 in use; where exp(log_decay) is 0 in float32 (-inf, the type's lowest value, anything
+    under -103.97) the (finite) state is cleared in front of its token, as where a row of the batch goes on with another episode. initial_state float32 [B, H, K, V] (None: zeros). lengths int32 [B] (None: T): tokens at and behind
     lengths[b] are not read and change nothing, their outputs and gradients are 0. scale: 1 / sqrt(K) where None. Keys have unit length in use:
     the rule needs beta |k|^2 < 2 to stay bounded.
 
-    Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 at -inf), beta and
+    Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 where it clears), beta and
     initial_state, once (no create_graph). The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32:
     (K V + 64 (K + V)) * 4 bytes."""
     plan = _check(q, k, v, log_decay, beta, initial_state, lengths, 2)
@@ -145,7 +145,7 @@ def _pack_step(plan, scale, q, k, v, g, beta):
 
 def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
     """One token of gated_delta_rule for every row: q, k [B, Hk, K], v [B, H, V], log_decay, beta float32 [B, H]; `state` float32 [B, H, K, V], contiguous,
-    is updated in place and shares no memory with the other arguments (log_decay = -inf: cleared first, whatever it holds). Returns out [B, H, V]. For acting: no gradients."""
+    is updated in place and shares no memory with the other arguments (cleared first, whatever it holds, where exp(log_decay) is 0). Returns out [B, H, V]. For acting: no gradients."""
     tensors((state, "the state"))
     plan = _check(q, k, v, log_decay, beta, state, None, 1)
     if not state.is_contiguous():

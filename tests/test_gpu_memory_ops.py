@@ -164,6 +164,29 @@ def test_delta_rule_on_strong_decays(ops, decay):
     check_delta(ops, delta_inputs(g, 2, 130, 2, 2, 32, 32, F32, decay=decay), randn(g, 2, 2, 32, 32))
 
 
+@pytest.mark.parametrize("low", [-103.0, -104.5, -200.0, -1e15, -1e30, torch.finfo(F32).min])
+@pytest.mark.parametrize("at", [(10,), (0, 70), (20, 40), (20, 21, 63, 64)])
+def test_delta_rule_on_finite_stand_ins_for_a_reset(ops, low, at):
+    """A gate whose exponential is 0 (or nearly) clears the state like -inf and leaves the gates behind it what they are; the one-token step agrees."""
+    g = gen(51)
+    inputs = delta_inputs(g, 2, 100, 2, 1, 24, 20, F32)
+    for t in at:
+        inputs[3][:, t, 0] = low
+    state = randn(g, 2, 2, 24, 20)
+    got = check_delta(ops, inputs, state)
+    if low < -104:
+        assert (got[3][:, list(at), 0] == 0).all()
+        as_inf = [x.clone() for x in inputs]
+        as_inf[3][as_inf[3] == low] = -INF
+        for x, y in zip(ops.gated_delta_rule(*inputs, initial_state=state), ops.gated_delta_rule(*as_inf, initial_state=state)):
+            assert torch.equal(x, y)
+    S, want = state.clone(), R.delta_rule(*[x.double() for x in inputs], state.double())
+    for t in range(100):
+        o = ops.gated_delta_step(*[x[:, t] for x in inputs], S)
+        R.close(o, want[0][:, t], 0, 4 * (t + 4) + 24 + 20, "step %d" % t, want[0].abs().max().item())
+    R.close(S, want[1], 0, 4 * 100 + 44, "state")
+
+
 def test_delta_rule_takes_slices_and_expanded_inputs(ops):
     """q, k and v as slices of one projection (rows of odd stride and start), gates expanded over the heads."""
     g = gen(6)
