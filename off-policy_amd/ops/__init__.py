@@ -8,7 +8,8 @@ rnn.py:5-43). These operators are what a wider or longer memory is made of:
     o = memory(q, k, v, log decay, beta)       gated_delta_rule (whole episodes, with gradients), gated_delta_step (one step of acting)
     x = o Wo^T + s                             linear with a residual
 
-float32, bfloat16 and float16; the gradients come through torch.autograd. Everything runs on the tensors' device and torch's current stream
+float32, bfloat16 and float16; the gradients come through torch.autograd, backwards and once: forward mode, torch.func's transforms, torch.jit.trace and
+make_fx are refused. Everything runs on the tensors' device and torch's current stream
 there, allocates through torch's allocator (so it may be captured into a HIP graph) and keeps nothing between calls. There is no CPU path.
 """
 from .memory import gated_delta_rule, gated_delta_step

@@ -6,6 +6,8 @@ that depends on a tensor's place or contents is."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental import proxy_tensor
 
 from .. import _lib
 
@@ -15,6 +17,7 @@ PLANS = 1024              # combinations of sizes and strides that are remembere
 _NONE = contextlib.nullcontext()
 grad_enabled = torch.is_grad_enabled
 stream = _lib.current_stream
+_transforms = torch._C._functorch.peek_interpreter_stack
 
 
 def dtype_code(dtype, name):
@@ -72,6 +75,29 @@ def like(t):
     return out if out.shape[-1] <= 1 or out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def plain_call(*ts):
+    """Refuses what torch.autograd's tape alone would get right: the kernels are called by address, so a tracer would record the outputs' allocation and
+    nothing that fills it (torch.jit.trace: untraced()), and a tangent (forward mode) or a batch axis (vmap) would be dropped."""
+    if forward_ad._current_level < 0 and proxy_tensor._CURRENT_MAKE_FX_TRACER is None and _transforms() is None:
+        return
+    if proxy_tensor._CURRENT_MAKE_FX_TRACER is not None:
+        raise RuntimeError("the memory operators cannot be recorded by make_fx")
+    for t in ts:
+        if t is None:
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError("the memory operators take no tensors inside torch.func transforms (vmap, grad, jvp): use torch.autograd")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the memory operators have no forward-mode derivative: a tensor with a tangent was given")
+
+
+def untraced():
+    """For what is worked out once for each combination of sizes: sizes are tensors while torch.jit.trace records, so such a call finds nothing kept and
+    comes here."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("the memory operators cannot be recorded by torch.jit.trace")
+
+
 def wants_grad(*ts):
     if grad_enabled():
         for t in ts:
@@ -86,6 +112,7 @@ def once(backward):
     def run(ctx, *grads):
         if grad_enabled():
             raise RuntimeError("the gradients of the memory operators cannot be differentiated again: no create_graph")
+        plain_call(*grads)
         return backward(ctx, *grads)
     return staticmethod(run)
 

@@ -5,7 +5,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import PLANS, dtype_code, inner, like, on_device, once, ptr, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import PLANS, dtype_code, inner, like, on_device, once, plain_call, ptr, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, untraced, wants_grad
 
 _CFG = struct.Struct("7if33q")
 _NONE3 = (0, 0, 0)
@@ -16,6 +16,7 @@ _lib_forward, _lib_backward, _lib_step = _lib.lib.ope_delta_forward, _lib.lib.op
 @functools.lru_cache(PLANS)
 def _plan(q, k, v, g, beta, state, lengths, dtypes, lead):
     """(B, T, H, Hk, K, V, type code) of shapes and types that fit together; `lead` axes in front of the heads (2: batch and time, 1: batch)."""
+    untraced()
     q_dtype, k_dtype, v_dtype, g_dtype, beta_dtype, state_dtype, lengths_dtype = dtypes
     code = dtype_code(q_dtype, "q")
     if len(q) != lead + 2 or len(v) != lead + 2 or v[:lead] != q[:lead]:
@@ -125,6 +126,7 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
     Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 where it clears), beta and
     initial_state, once (no create_graph). The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32:
     (K V + 64 (K + V)) * 4 bytes."""
+    plain_call(q, k, v, log_decay, beta, initial_state)
     plan = _check(q, k, v, log_decay, beta, initial_state, lengths, 2)
     scale = float(plan[4] ** -0.5 if scale is None else scale)
     with on_device(q, k, v, log_decay, beta, initial_state, lengths):
@@ -146,6 +148,7 @@ def _pack_step(plan, scale, q, k, v, g, beta):
 def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
     """One token of gated_delta_rule for every row: q, k [B, Hk, K], v [B, H, V], log_decay, beta float32 [B, H]; `state` float32 [B, H, K, V], contiguous,
     is updated in place and shares no memory with the other arguments (cleared first, whatever it holds, where exp(log_decay) is 0). Returns out [B, H, V]. For acting: no gradients."""
+    plain_call(q, k, v, log_decay, beta, state)
     tensors((state, "the state"))
     plan = _check(q, k, v, log_decay, beta, state, None, 1)
     if not state.is_contiguous():

@@ -5,7 +5,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, plain_call, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, untraced, wants_grad
 
 _CFG = struct.Struct("qqqiiif")
 _MAX_WIDTH = 1 << 20
@@ -25,6 +25,7 @@ def _bwd_bytes(cfg):
 @functools.lru_cache(PLANS)
 def _plan(x, x_dtype, w, w_dtype, r, r_dtype, eps):
     """(type code, rows, width) of shapes and types that fit together."""
+    untraced()
     code = dtype_code(x_dtype, "x")
     if len(x) < 1 or not 1 <= x[-1] <= _MAX_WIDTH:
         raise ValueError("x: at least one axis and a last one of 1 to %d wanted, got shape %s" % (_MAX_WIDTH, tuple(x)))
@@ -110,6 +111,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     x [..., D] float32, bfloat16 or float16, weight [D] and residual (x's shape) of the same type. Returns y, or (y, s) where a residual is
     given: s is what the next block adds to. The norm is taken of the float32 sum, in front of its rounding to x's type. Differentiable in x,
     weight and residual, once (no create_graph)."""
+    plain_call(x, weight, residual)
     eps = float(eps)
     plan = _check(x, weight, residual, eps)
     with on_device(x, weight, residual):
@@ -123,6 +125,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     """rms_norm with its output in 8 bits: returns (q, scale), or (q, scale, s) where a residual is given. q is float8_e4m3fn of x's shape, scale
     float32 of x.shape[:-1], y = q * scale; scale = max(max|y|, 448 * 2^-126) / 448 of the row. For acting: no gradients (a tensor that requires one
     is refused while gradients are recorded)."""
+    plain_call(x, weight, residual)
     eps = float(eps)
     plan = _check(x, weight, residual, eps)
     if wants_grad(x, weight, residual):
@@ -134,6 +137,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
 
 def quantize_rows_fp8(x):
     """(q, scale) of the rows of x [..., D], by rms_norm_fp8's rule; for the weights of linear_fp8."""
+    plain_call(x)
     tensors((x, "x"))
     code, M, D = _plan(x.shape, x.dtype, None, None, None, None, 0.0)
     if wants_grad(x):

@@ -5,7 +5,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, wants_grad
+from ._common import DTYPES, E4M3, PLANS, dtype_code, on_device, once, plain_call, ptr, rows_of, same_dtype, same_shape, scratch, size_or_raise, stream, tensors, untraced, wants_grad
 
 ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "silu": 3, "gelu": 4}
 _CFG = struct.Struct("qqqiiiii4x")
@@ -28,6 +28,7 @@ def _bwd_bytes(cfg):
 @functools.lru_cache(PLANS)
 def _plan(x, x_dtype, w, w_dtype, b, b_dtype, r, r_dtype, activation, out_dtype):
     """(rows, in, out, activation, type code, type code of the output) of shapes and types that fit together."""
+    untraced()
     if out_dtype not in DTYPES:
         raise TypeError("out_dtype: float32, bfloat16 or float16 wanted, got %s" % (out_dtype,))
     same_dtype(w_dtype, "weight", x_dtype)
@@ -116,6 +117,7 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     x [..., in], weight [out, in] (torch.nn.Linear's), bias [out], residual [..., out], all of one type (float32, bfloat16 or float16); activation
     "none", "relu", "tanh", "silu" or "gelu" (z Phi(z)). Sums in float32, one rounding at the end. Differentiable in all four, once (no create_graph); the gradient of
     z = x weight^T + bias is rounded to x's type in front of the backward products."""
+    plain_call(x, weight, bias, residual)
     tensors((x, "x"))
     dtype_code(x.dtype, "x")
     plan = _check(x, weight, bias, residual, activation, x.dtype)
@@ -129,6 +131,7 @@ def linear_fp8(x, x_scale, weight, w_scale, bias=None, residual=None, activation
     """y = act((x weight^T) x_scale w_scale + bias) + residual with 8-bit operands, as rms_norm_fp8 and quantize_rows_fp8 return them: x [..., in]
     and weight [out, in] float8_e4m3fn, x_scale float32 of x.shape[:-1], w_scale float32 [out]; bias and residual of out_dtype. For acting: no gradients
     (an argument that requires one is refused while gradients are recorded)."""
+    plain_call(x, x_scale, weight, w_scale, bias, residual)
     tensors((x, "x"), (x_scale, "x_scale"), (w_scale, "w_scale"))
     same_dtype(x.dtype, "x", E4M3)
     plan = _check(x, weight, bias, residual, activation, out_dtype)

@@ -812,6 +812,36 @@ def test_changed_inputs_are_noticed(ops):
             y.sum().backward()
 
 
+def test_a_compiled_program_calls_the_kernels(ops):
+    """torch.compile leaves the calls to Python: same results, new inputs seen, gradients too."""
+    torch._dynamo.reset()
+    g = gen(52)
+    w, n = randn(g, 24, 16), randn(g, 16)
+
+    def f(x, r):
+        y, s = ops.rms_norm(x * 2, n, residual=r)
+        return ops.linear(y, w, activation="silu") + s.sum(-1, keepdim=True)
+
+    c = torch.compile(f, backend="eager")
+    for _ in range(3):
+        x, r = randn(g, 70, 16), randn(g, 70, 16)
+        with torch.no_grad():
+            assert torch.equal(c(x, r), f(x, r))
+        a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(c(a, r).sum(), a)[0], torch.autograd.grad(f(b, r).sum(), b)[0])
+    torch._dynamo.reset()
+
+
+def test_tangents_in_the_gradients_are_refused(ops):
+    from torch.autograd import forward_ad
+    x, w = torch.ones(70, 8, device="cuda", requires_grad=True), torch.ones(5, 8, device="cuda")
+    y = ops.linear(x, w)
+    with forward_ad.dual_level():
+        dy = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, dy)
+
+
 def test_tensors_on_two_devices_are_refused(ops):
     x, w = torch.zeros(3, 8, device="cuda"), torch.zeros(8)
     with pytest.raises(ValueError, match="in one call"):

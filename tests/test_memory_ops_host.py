@@ -98,6 +98,61 @@ def test_acting_forms_refuse_arguments_that_want_gradients():
         ops.quantize_rows_fp8(torch.zeros(3, 8, requires_grad=True))
 
 
+def entries():
+    """Every entry point as a function of one float32 tensor [3, 8] that it reads, on the CPU: a call that is not refused first ends with "GPU only"."""
+    w, xs, ws = torch.zeros(5, 8), torch.ones(3), torch.ones(5)
+    d, s = delta_args(B=1, T=3, Hk=1, H=1, K=8, V=8), delta_args(B=3, Hk=1, H=1, K=8, V=8, step=True)
+    return {
+        "rms_norm": lambda x: ops.rms_norm(x, w[0]), "rms_norm, residual": lambda x: ops.rms_norm(w[:3], w[0], residual=x), "rms_norm_fp8": lambda x: ops.rms_norm_fp8(x, w[0]),
+        "quantize_rows_fp8": lambda x: ops.quantize_rows_fp8(x), "linear": lambda x: ops.linear(x, w), "linear, weight": lambda x: ops.linear(w, x),
+        "linear, residual": lambda x: ops.linear(w[:3], torch.zeros(8, 8), residual=x),
+        "linear_fp8, residual": lambda x: ops.linear_fp8(w[:3].to(E4M3), xs, torch.zeros(8, 8).to(E4M3), torch.ones(8), residual=x, out_dtype=F32),
+        "linear_fp8, scale": lambda x: ops.linear_fp8(w[:3].to(E4M3), x[:, 0], w.to(E4M3), ws),
+        "gated_delta_rule": lambda x: ops.gated_delta_rule(d[0], d[1], x[None, :, None], d[3], d[4]),
+        "gated_delta_rule, state": lambda x: ops.gated_delta_rule(*d, initial_state=x[None, None, :1].expand(1, 1, 8, 8)),
+        "gated_delta_step": lambda x: ops.gated_delta_step(x[:, None], s[1], s[2], s[3], s[4], torch.zeros(3, 1, 8, 8)),
+    }
+
+
+@pytest.mark.parametrize("name", list(entries()))
+def test_what_the_tape_does_not_see_is_refused(name):
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x = entries()[name], torch.zeros(3, 8)
+    first = lambda y: y[0] if isinstance(y, tuple) else y         # noqa: E731
+    with pytest.raises(ValueError, match="GPU only"):              # an ordinary call passes these checks
+        f(x)
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(ValueError, match="GPU only"):          # no tangent, no harm
+            f(x)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match="jit.trace"), torch.no_grad():
+        torch.jit.trace(lambda x: first(f(x)), (x,), check_trace=False)
+    for pre in (False, True):
+        with pytest.raises(RuntimeError, match="make_fx"):
+            make_fx(lambda x: first(f(x)), pre_dispatch=pre)(x)
+    for transform in (lambda: torch.func.vmap(f)(torch.zeros(2, 3, 8)), lambda: torch.func.grad(lambda x: first(f(x)).sum())(x),
+                      lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.functionalize(f)(x)):
+        with pytest.raises(RuntimeError, match="torch.func"):
+            transform()
+
+
+def test_a_tangent_in_the_gradients_is_refused():
+    """Forward over reverse: the backward pass would drop it."""
+    from torch.autograd import forward_ad
+    from offpolicy_amd.ops import _common
+    seen = []
+    backward = _common.once(lambda ctx, *grads: seen.append(grads)).__func__
+    x = torch.ones(3)
+    with torch.no_grad(), forward_ad.dual_level():
+        backward(None, x, None)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            backward(None, None, forward_ad.make_dual(x, x))
+    assert len(seen) == 1
+
+
 def test_there_is_no_cpu_path():
     with pytest.raises(ValueError, match="GPU only"):
         ops.gated_delta_rule(*delta_args())
