@@ -142,7 +142,7 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
 def _pack_step(plan, scale, q, k, v, g, beta):
     _, _, H, _, _, V, _ = plan
     three = lambda s: (s[0], 0, s[1])       # noqa: E731
-    return _CFG.pack(*plan, float(plan[4] ** -0.5 if scale is None else scale), *three(q), *three(k), *three(v), H * V, 0, V, *three(g), *three(beta), *_NONE3 * 5)
+    return _CFG.pack(*plan, scale, *three(q), *three(k), *three(v), H * V, 0, V, *three(g), *three(beta), *_NONE3 * 5)
 
 
 def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
@@ -151,6 +151,7 @@ def gated_delta_step(q, k, v, log_decay, beta, state, scale=None):
     plain_call(q, k, v, log_decay, beta, state)
     tensors((state, "the state"))
     plan = _check(q, k, v, log_decay, beta, state, None, 1)
+    scale = float(plan[4] ** -0.5 if scale is None else scale)
     if not state.is_contiguous():
         raise ValueError("the state is updated in place and has to be contiguous")
     if wants_grad(q, k, v, log_decay, beta, state):

@@ -292,6 +292,15 @@ def test_delta_step(ops, B, H, Hk, K, V, dtype):
         R.close(mine, S64, 0, 3 * n, "state")
 
 
+def test_delta_step_reads_its_scale_in_every_call(ops):
+    """A scale that is a tensor is taken by its value, not by which tensor it is."""
+    a = [x[:, 0] for x in delta_inputs(gen(53), 2, 1, 2, 2, 16, 16, F32)]
+    scale, S = torch.tensor(0.5), torch.zeros(2, 2, 16, 16, device="cuda")
+    one = ops.gated_delta_step(*a, S.clone(), scale=scale)
+    scale.fill_(2.0)
+    assert torch.equal(ops.gated_delta_step(*a, S.clone(), scale=scale), 4 * one) and torch.equal(ops.gated_delta_step(*a, S.clone(), scale=2), 4 * one)
+
+
 def test_delta_steps_follow_the_chunked_pass(ops):
     g = gen(10)
     inputs = delta_inputs(g, 3, 90, 2, 1, 48, 40, F32, 0.03)
