@@ -96,29 +96,49 @@ __device__ __forceinline__ u32x4 last16(const uint8_t* row, int64_t half, int g,
   return v;
 }
 
-// 1 / (1 + e^-z) by the hardware's 2^x and 1/x, each within one step of float32: with expf and a division the epilogue of a 4096 x 4096 output took
-// 20 us more than without an activation. e^-z past the range is infinite, its reciprocal 0.
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
+// e^-z and s = 1 / (1 + e^-z) by the hardware's 2^x and 1/x, each within one step of float32: with expf and a division the epilogue of a 4096 x 4096
+// output took 20 us more than without an activation. e^-z past the range is infinite, its reciprocal 0. The rounding of the exponent z log2 e alone moves e^-z
+// by |z| 2^-24 of itself: nothing beside the rounding of a 16-bit result, up to 64 half steps of a float32 one. WIDE (float32 results) makes that good
+// with the exponent's low part, where e^-z is in range.
+template <bool WIDE>
+__device__ __forceinline__ float sigmoid(float z, float* ez = nullptr) {
+  constexpr float L = -1.44269504088896341f, Llo = (float)(-1.44269504088896341 - (double)L);
+  const float t = z * L;
+  float e = __builtin_amdgcn_exp2f(t);
+  if (WIDE) {
+    const float low = fmaf(z, Llo, fmaf(z, L, -t)) * 0.69314718055994531f;
+    e = fabsf(z) < 88.f ? fmaf(e, low, e) : e;
+  }
+  if (ez) *ez = e;
+  return __builtin_amdgcn_rcpf(1.f + e);
+}
+template <bool WIDE>
 __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
     case OPE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
     case OPE_ACT_TANH: return tanhf(z);
-    case OPE_ACT_SILU: return z * sigmoid(z);
+    case OPE_ACT_SILU: return z * sigmoid<WIDE>(z);
     case OPE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
   }
   return z;
 }
+template <bool WIDE>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case OPE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case OPE_ACT_TANH: { const float t = tanhf(z); return 1.f - t * t; }
-    case OPE_ACT_SILU: { const float s = sigmoid(z); return s * (1.f + z * (1.f - s)); }
+    case OPE_ACT_SILU: {
+      float e;
+      const float s = sigmoid<WIDE>(z, &e);
+      return s * (1.f + z * (WIDE && z > 0.f ? e * s : 1.f - s));       // (1 - s = e^-z s, which keeps its bits where s is next to 1)
+    }
     case OPE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
   }
   return 1.f;
 }
+template <bool WIDE>
 __device__ __forceinline__ f32x4 act4(f32x4 z, int act) {          // one branch for the four
-  const auto each = [&](auto a) { return f32x4{act_of(z[0], a()), act_of(z[1], a()), act_of(z[2], a()), act_of(z[3], a())}; };
+  const auto each = [&](auto a) { return f32x4{act_of<WIDE>(z[0], a()), act_of<WIDE>(z[1], a()), act_of<WIDE>(z[2], a()), act_of<WIDE>(z[3], a())}; };
   switch (act) {
     case OPE_ACT_RELU: return each(std::integral_constant<int, OPE_ACT_RELU>{});
     case OPE_ACT_TANH: return each(std::integral_constant<int, OPE_ACT_TANH>{});
@@ -158,7 +178,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, f32x4 acc, int64_t m,
   }
   if (e.x_scale) z *= sw * e.x_scale[m];
   z += b;
-  const f32x4 y = act4(z, e.act) + res;
+  const f32x4 y = act4<sizeof(O) == 4>(z, e.act) + res;
   const int64_t at = m * e.N + n;
   if (live == 4) {
     store_pack<O, 4>((O*)e.y + at, y);
@@ -459,7 +479,7 @@ __global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const
       if (m >= M) break;
       if constexpr (ACT != OPE_ACT_NONE) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) d[i][c] *= act_slope(x[i][c], ACT);
+        for (int c = 0; c < 4; ++c) d[i][c] *= act_slope<sizeof(T) == 4>(x[i][c], ACT);
         store_pack<T, 4>(dz + m * N + n, d[i]);
       }
       s += d[i];
@@ -473,7 +493,7 @@ __global__ __launch_bounds__(256) void linear_dz(const T* __restrict__ dy, const
         if (n + c < N) {
           float d = (float)dy[m * N + n + c];
           if constexpr (ACT != OPE_ACT_NONE) {
-            d *= act_slope(z[m * N + n + c], ACT);
+            d *= act_slope<sizeof(T) == 4>(z[m * N + n + c], ACT);
             dz[m * N + n + c] = (T)d;
           }
           s[c] += d;

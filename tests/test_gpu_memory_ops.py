@@ -542,6 +542,26 @@ def test_linear_tiles_of_every_size(ops, M, K, N, dtype):
     check_linear(ops, gen(48), M, K, N, dtype, "silu")
 
 
+@pytest.mark.parametrize("rows", [64, 60001])
+def test_silu_and_its_slope_keep_their_bits_in_float32(ops, rows):
+    """z passes through unchanged (a width of 1, weight 1). e^-z is off by 2 half steps (one step of the exponential) and its correction's rounding, 1 + e^-z
+    by one more, the reciprocal by 2, the product by 1: 7; the slope s (1 + z (1 - s)) twice that of the size of its two terms. Down to -87: the
+    sigmoid is subnormal below."""
+    g = gen(54)
+    z = torch.cat([torch.linspace(-87, 87, rows // 2, device="cuda"), randn(g, rows - rows // 2, scale=4.0).clamp(-87, 87)])[:, None].requires_grad_()
+    y = ops.linear(z, torch.ones(1, 1, device="cuda"), activation="silu")
+    z64 = z.detach().double()
+    s64 = torch.sigmoid(z64)
+    assert ((y.double() - z64 * s64).abs() <= 8 * R.U32 * (z64 * s64).abs()).all()
+    slope = torch.autograd.grad(y, z, torch.ones_like(y))[0].double()
+    assert ((slope - s64 * (1 + z64 * (1 - s64))).abs() <= 16 * R.U32 * (s64 + (z64 * s64 * (1 - s64)).abs())).all()
+    far = torch.tensor([[100.0], [1e30], [INF], [-100.0], [-1e30], [math.nan]], device="cuda", requires_grad=True)
+    y = ops.linear(far, torch.ones(1, 1, device="cuda"), activation="silu")
+    assert torch.equal(y[:3], far[:3]) and (y[3:5].abs() < 1e-36).all() and torch.isnan(y[5])
+    slope = torch.autograd.grad(y, far, torch.ones_like(y))[0]
+    assert (slope[:2] == 1).all() and (slope[3:5].abs() < 1e-36).all()
+
+
 def in_order(x, w, order):
     """x w^T in float32, one fused multiply-add for each k of `order` (a product of two float32 values is exact in 64 bits)."""
     acc = torch.zeros(x.shape[0], w.shape[0], device="cuda")
