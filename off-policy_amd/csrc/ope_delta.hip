@@ -275,7 +275,8 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 4) void delta_out(op
     acc += acc2;
     acc = turn4(acc);                      // four columns of one token a lane
     const int tt = 16 * w + 4 * g + (j & 3), v4 = 16 * vt + 4 * (j >> 2);
-    if (tt < rows) {                       // (rows behind the last live token: q = 0, and so is this)
+    if (tt >= a.nv) acc = f32x4{0.f, 0.f, 0.f, 0.f};   // (behind the last live token q is 0, but its product with a state that is not finite is not)
+    if (tt < rows) {
       T* p = o0 + (int64_t)tt * cfg.o_stride[1] + v4;
       if (v4 + 4 <= d.V) store_pack<T, 4>(p, acc);
       else

@@ -107,9 +107,11 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   T* dv0 = dv + a.b * cfg.dv_stride[0] + (int64_t)a.t0 * cfg.dv_stride[1] + a.h * cfg.dv_stride[2];
   float* dg0 = dg + a.b * cfg.dg_stride[0] + (int64_t)a.t0 * cfg.dg_stride[1] + a.h * cfg.dg_stride[2];
   float* db0 = dbeta + a.b * cfg.dbeta_stride[0] + (int64_t)a.t0 * cfg.dbeta_stride[1] + a.h * cfg.dbeta_stride[2];
-  // four elements of dq / dk at (t, f): of the type itself, or this value head's float32 share
+  // four elements of dq / dk at (t, f): of the type itself, or this value head's float32 share. 0 behind the last live token: what was computed there is
+  // 0 times a state, which need not be finite.
   auto put_k = [&](T* out, const int64_t* stride, float* share, int t, int f, f32x4 x) {
     if (t >= rows) return;
+    if (t >= a.nv) x = f32x4{0.f, 0.f, 0.f, 0.f};
     if (own) {
       T* p = out + a.b * stride[0] + (int64_t)(a.t0 + t) * stride[1] + hk * stride[2] + f;
       if (f + 4 <= d.K) store_pack<T, 4>(p, x);
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     for (int is = 0; is < 4; ++is)
       if (is <= wt) M[is] = mfma4(tile(2 * KT + is), bm, M[is]);
     if ((vt & 1) == half) {                            // one half writes dv and counts dR.v
-      const f32x4 y = r * gt.beta[t];
+      const f32x4 y = t < a.nv ? r * gt.beta[t] : f32x4{0.f, 0.f, 0.f, 0.f};
       rv += r[0] * x[0] + r[1] * x[1] + r[2] * x[2] + r[3] * x[3];
       T* p = dv0 + (int64_t)t * cfg.dv_stride[1] + v;
       if (t < rows) {

@@ -127,6 +127,24 @@ def test_delta_rule_on_ragged_rows(ops, dtype):
     assert (o[dead] == 0).all() and torch.equal(S[0], state[0]) and torch.equal(S[7], state[7])
 
 
+@pytest.mark.parametrize("value", [math.nan, INF])
+@pytest.mark.parametrize("Hk,dtype", [(2, F32), (1, BF16)])
+def test_behind_the_length_all_is_zero_whatever_the_state_holds(ops, Hk, dtype, value):
+    g = gen(55)
+    lengths = torch.tensor([0, 1, 40, 64, 70, 100], dtype=torch.int32, device="cuda")
+    B, T = len(lengths), 100
+    inputs = delta_inputs(g, B, T, 2, Hk, 24, 20, dtype)
+    state = randn(g, B, 2, 24, 20)
+    state[:, 0, 3] = value
+    leaves = [x.detach().requires_grad_() for x in inputs] + [state.requires_grad_()]
+    o, S = ops.gated_delta_rule(*leaves[:5], initial_state=state, lengths=lengths)
+    grads = torch.autograd.grad([o, S], leaves, [randn(g, B, T, 2, 20, dtype=dtype), randn(g, B, 2, 24, 20)])
+    dead = torch.arange(T, device="cuda")[None] >= lengths[:, None]
+    for x in (o, *grads[:5]):
+        assert (x[dead] == 0).all()
+    assert torch.equal(S[0].isnan(), state[0].isnan()) and not o[1:, 0, 0].isfinite().all()
+
+
 def test_delta_rule_resets_are_exact(ops):
     """A row that holds two episodes gives, behind the reset, bit for bit what the second one gives at the same place of its chunk after another first."""
     g = gen(3)
