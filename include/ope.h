@@ -732,7 +732,8 @@ int ope_quantize_rows(const ope_norm_cfg* cfg, const void* x, void* q, float* sc
  *         of n_qk_heads: query / key head i serves the value heads [i * r, (i + 1) * r), r = n_heads / n_qk_heads.
  *   g     float32, log of the decay, beta float32: [batch][seq_len][n_heads], strides g_stride / beta_stride.
  *         Where e^g is 0 in float32 (-inf, the type's lowest value, anything under -103.97) the state is cleared in front of the token (an
- *         episode boundary inside a row).
+ *         episode boundary inside a row), whatever it holds: what is not finite in one episode of a row, its gradients among it, reaches no other
+ *         episode. Inside its own it may also reach tokens in front of it, within their 64.
  *   lengths  int32 [batch] or NULL: tokens t >= lengths[b] (clamped to [0, seq_len]) are neither read nor do anything; their o is 0.
  *   state0   float32 [batch][n_heads][key_dim][value_dim] or NULL (zeros); state_out the same shape: the state behind the last live token.
  * The forward pass works on chunks of 64 tokens: with G the running sum of g inside a chunk, A_ij = beta_i exp(G_i - G_j) k_i.k_j (i > j),

@@ -12,7 +12,8 @@
 //   ST [c][VT][KT]  S  the state in front of the chunk: rows v, columns k
 //   UT [c][VT][4]   S  U0 before the scan, u of the chunk's tokens after it: rows v, columns t
 //   WT [c][KT][4]   S  W transposed: rows k, columns t
-//   gC [c]          S  decay over the whole chunk (0 behind a reset);   tails [c][64]  S  decay from t to the chunk's end
+//   gC [c]          S  decay over the whole chunk (0 behind a reset);   tails [c][64]  S  decay from t to the chunk's end, with a minus sign where a
+//                      reset lies between the chunk's start and t
 //   W  [c][4][KT]   W  rows t, columns k;   KTs [c][KT][4]  W  of the inputs' type: k transposed, rows k, columns t
 //   backward: Ks [c][4][KT]  W  of the inputs' type: k, rows t, columns k;   dUT like UT (dU0, then dU, then dR with its tiles transposed);
 //   dST like ST (N, then the gradient of the state BEHIND the chunk);   dqp, dkp [b][t][H][K] where query / key heads are shared
@@ -66,11 +67,42 @@ __device__ __forceinline__ ChunkAt chunk_at(const DeltaDims& d, const int32_t* l
 // keep their last bits); a reset (e^g = 0 in float32: -inf, and every g under -103.97, so that no finite stand-in for -inf swallows the small gates
 // that are added behind it) starts a new segment with G = 0, and decays across segments are exactly 0: what lies behind a reset
 // does not depend on what lies in front of it, to the last bit.
+//
+// Nor does it where values are not finite. A product by a mask's zeros lets them through (0 times NaN), so (1) what a decay scales is dropped where the
+// decay is 0 (gated), and (2) a matrix product whose contraction runs over the tokens of several segments is done again one segment at a time where
+// its result is not finite (only), or goes without the values that are not (delta_bwd_main). That costs the few chunks it happens in; without a reset in
+// the chunk nothing is asked. Inside its segment such a value may spread to the chunk's tokens in front of it.
 struct Gates {
   float hi[kC], lo[kC], beta[kC], head[kC], tail[kC];   // head: decay from the chunk's start through t; tail: from t to its end
   int seg[kC];
   float whole;                                          // decay over the whole chunk
+  __device__ __forceinline__ int first() const { return __builtin_amdgcn_readfirstlane(seg[0]); }
+  __device__ __forceinline__ int last() const { return __builtin_amdgcn_readfirstlane(seg[kC - 1]); }      // 0: no reset in the chunk
 };
+__device__ __forceinline__ float gated(float decay, float x) { return decay == 0.f ? 0.f : decay * x; }
+__device__ __forceinline__ f32x4 gated(f32x4 decay, f32x4 x) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = gated(decay[r], x[r]);
+  return x;
+}
+// x of the tokens t .. t + 3, 0 where they belong to another segment than s. (The index is opaque: left to itself the compiler reads the segments of every
+// use far ahead, on the way that hardly ever comes here too, and spills.)
+__device__ __forceinline__ f32x4 only(const Gates& gt, int s, int t, f32x4 x) {
+  asm volatile("" : "+v"(t));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = gt.seg[t + r] == s ? x[r] : 0.f;
+  return x;
+}
+// Whether all of x[0 .. N) are finite, by one sum (where that alone leaves the range, no: asked again at no harm). z - z is 0 for finite numbers alone.
+template <int N>
+__device__ __forceinline__ bool finite(const f32x4* x) {
+  f32x4 z = x[0];
+#pragma unroll
+  for (int n = 1; n < N; ++n) z += x[n];
+  const float s = (z[0] + z[1]) + (z[2] + z[3]);
+  return s - s == 0.f;
+}
+__device__ __forceinline__ bool finite(f32x4 x) { return finite<1>(&x); }
 __device__ __forceinline__ float decay(const Gates& s, int t, int u) {   // from u through t (u <= t)
   return s.seg[t] == s.seg[u] ? expf((s.hi[t] - s.hi[u]) + (s.lo[t] - s.lo[u])) : 0.f;
 }
@@ -231,15 +263,17 @@ __device__ __forceinline__ void minus_A(float (*NA)[kC + 4], const Rows<T, KT>& 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int s = 16 * is + 4 * g + r;
-      acc[r] = s < t ? -gt.beta[t] * decay(gt, t, s) * acc[r] : 0.f;
+      const float d = decay(gt, t, s);
+      acc[r] = s < t && d != 0.f ? -gt.beta[t] * d * acc[r] : 0.f;
     }
     put4(&NA[t][16 * is + 4 * g], acc);
   }
 }
 // Inverses of the four unit lower triangular 16 x 16 blocks on the diagonal of I + A, by forward substitution: lane (column c, block). One wave.
-__device__ __forceinline__ void diag_inverse(float (*inv)[16][20], const float (*NA)[kC + 4]) {
+__device__ __forceinline__ void diag_inverse(float (*inv)[16][20], const float (*NA)[kC + 4], const Gates& gt) {
   const int c = threadIdx.x & 15, blk = (threadIdx.x >> 4) & 3;
   float t[16];
+  bool fine = true;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float v = i == c ? 1.f : 0.f;
@@ -252,6 +286,18 @@ __device__ __forceinline__ void diag_inverse(float (*inv)[16][20], const float (
           if (4 * q + r < i) v = fmaf(a[r], t[4 * q + r], v);
       }
     t[i] = v;
+    fine &= v - v == 0.f;
+    inv[blk][i][c] = v;
+  }
+  if (gt.last() == 0 || !__any(!fine)) return;
+  // rows of A that are not finite: again, with the zeros above the diagonal and between segments kept
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    float v = i == c ? 1.f : 0.f;
+    if (i > c && gt.seg[16 * blk + i] == gt.seg[16 * blk + c])
+#pragma unroll 1
+      for (int q = c; q < i; ++q)
+        if (gt.seg[16 * blk + q] == gt.seg[16 * blk + c]) v = fmaf(NA[16 * blk + i][16 * blk + q], inv[blk][q][c], v);
     inv[blk][i][c] = v;
   }
 }

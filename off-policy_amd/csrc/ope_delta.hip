@@ -36,42 +36,75 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
   __syncthreads();
   minus_A<T, KT>(NA, k, gt);
   if (threadIdx.x == 0) gC[a.c] = gt.whole;
-  if (threadIdx.x < kC) tails[a.c * kC + threadIdx.x] = gt.tail[threadIdx.x];
+  if (threadIdx.x < kC) tails[a.c * kC + threadIdx.x] = copysignf(gt.tail[threadIdx.x], gt.seg[threadIdx.x] ? -1.f : 1.f);
   __syncthreads();
-  if (w == 0) diag_inverse(inv, NA);
-  for (int x = w; x < 4 * KT; x += NW) {                 // k transposed, a tile a wave
+  if (w == 0) diag_inverse(inv, NA, gt);
+  for (int x = w; x < 4 * KT; x += NW) {                 // k transposed, a tile a wave; 0 where the token does not reach the chunk's end
     const int kt = x >> 2, it = x & 3;
     typename Pack<T, 4>::vec v;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = k.v[16 * it + 4 * g + r][16 * kt + j];
+    for (int r = 0; r < 4; ++r) v[r] = gt.tail[16 * it + 4 * g + r] == 0.f ? (T)0.f : k.v[16 * it + 4 * g + r][16 * kt + j];
     *reinterpret_cast<typename Pack<T, 4>::vec*>(KTs + (a.c * KT * 4 + x) * 256 + tile_lane()) = v;
   }
   __syncthreads();
-  for (int cg = w; cg < KT + d.VT; cg += NW) {
-    f32x4 x[4];
-    const int col = cg < KT ? 16 * cg + j : 16 * (cg - KT) + j;
+  auto put = [&](int cg, int it, f32x4 x) {
+    if (cg < KT) {
+      put4(&WT[((a.c * KT + cg) * 4 + it) * 256 + tile_lane()], x);
+      put4(&W[((a.c * 4 + it) * KT + cg) * 256 + turned_lane()], turn4(x));
+    } else {
+      put4(&UT[((a.c * d.VT + cg - KT) * 4 + it) * 256 + tile_lane()], x);
+    }
+  };
+  auto right = [&](int cg, f32x4* x) {                   // the right-hand side
     if (cg < KT) {
 #pragma unroll
-      for (int it = 0; it < 4; ++it) x[it] = column4(&k.v[16 * it + 4 * g][col], Rows<T, KT>::kStride) * at4(&gt.head[16 * it + 4 * g]) * at4(&gt.beta[16 * it + 4 * g]);
+      for (int it = 0; it < 4; ++it)
+        x[it] = gated(at4(&gt.head[16 * it + 4 * g]), column4(&k.v[16 * it + 4 * g][16 * cg + j], Rows<T, KT>::kStride) * at4(&gt.beta[16 * it + 4 * g]));
     } else {
-      load_columns(x, v_in, cfg.v_stride, a, col, d.V);
+      load_columns(x, v_in, cfg.v_stride, a, 16 * (cg - KT) + j, d.V);
 #pragma unroll
       for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.beta[16 * it + 4 * g]);
     }
+  };
+  const int last = gt.last();
+  unsigned again = 0;                                    // this wave's column groups with something that is not finite
+  int mine = 0;
+  for (int cg = w; cg < KT + d.VT; cg += NW, ++mine) {
+    f32x4 x[4];
+    right(cg, x);
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
       f32x4 acc = x[it];
 #pragma unroll
       for (int kt = 0; kt < it; ++kt) acc = mfma4(at4(&NA[16 * it + j][16 * kt + 4 * g]), x[kt], acc);
       x[it] = mfma4(at4(&inv[it][j][4 * g]), acc, f32x4{0.f, 0.f, 0.f, 0.f});
-      if (cg < KT) {
-        put4(&WT[((a.c * KT + cg) * 4 + it) * 256 + tile_lane()], x[it]);
-        put4(&W[((a.c * 4 + it) * KT + cg) * 256 + turned_lane()], turn4(x[it]));
-      } else {
-        put4(&UT[((a.c * d.VT + cg - KT) * 4 + it) * 256 + tile_lane()], x[it]);
-      }
+      put(cg, it, x[it]);
     }
+    if (last && __any(!finite<4>(x))) again |= 1u << mine;
   }
+  if (!again) return;
+  mine = 0;
+#pragma unroll 1
+  for (int cg = w; cg < KT + d.VT; cg += NW, ++mine)
+    if (again >> mine & 1) {
+      f32x4 b[4], x[4] = {};
+      right(cg, b);
+#pragma unroll 1
+      for (int s = gt.first(); s <= (cg < KT ? 0 : last); ++s) {      // one segment at a time (W is 0 behind a reset, whatever A holds there)
+        f32x4 y[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          f32x4 acc = only(gt, s, 16 * it + 4 * g, b[it]);
+#pragma unroll
+          for (int kt = 0; kt < it; ++kt) acc = mfma4(at4(&NA[16 * it + j][16 * kt + 4 * g]), y[kt], acc);
+          acc = only(gt, s, 16 * it + 4 * g, acc);
+          y[it] = only(gt, s, 16 * it + 4 * g, mfma4(at4(&inv[it][j][4 * g]), acc, f32x4{0.f, 0.f, 0.f, 0.f}));
+          x[it] += y[it];
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) put(cg, it, x[it]);
+    }
 }
 
 // The scan, forward or backward in time. Four waves share 16 value columns of one (sequence, head): wave w makes the 16 tokens 16w.. of
@@ -81,6 +114,8 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
 //   forward : U = U0 - W S;            S' = gC S + k^T (tail U)          M1 = W (float32),   M2 = KTs
 //   backward: dU = dU0 + tail (k dS'); dS = gC dS' + N - WT dU           M1 = Ks,            M2 = WT (float32)
 // (a row of tail scales a product's result or its operand: the keys themselves stay in their own type, at half the bytes.)
+// A token behind a reset in its chunk (a minus sign on its tail) sees nothing of the state in front of the chunk and passes nothing back to it; one whose tail
+// is 0, nothing of the state behind it: what is not finite does not get through either.
 template <typename T, int KT, bool BWD>
 struct ScanOperands {
   static constexpr int NK = (KT + 3) / 4;             // tiles of keys a wave
@@ -151,8 +186,15 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
       get1(o, next, q);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const f32x4 u = BWD ? o.u + o.tail * (p0 + p1) : o.u - (p0 + p1);
-    put4(&UL[j][16 * w + 4 * g], BWD ? u : u * o.tail);
+    f32x4 u, pass;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool behind = __float_as_uint(o.tail[r]) >> 31;
+      const float tail = fabsf(o.tail[r]), p = p0[r] + p1[r];
+      u[r] = BWD ? o.u[r] + gated(tail, p) : (behind ? o.u[r] : o.u[r] - p);
+      pass[r] = BWD ? (behind ? 0.f : u[r]) : gated(tail, u[r]);
+    }
+    put4(&UL[j][16 * w + 4 * g], pass);
     put4(&UT[((c * VT + vt) * 4 + w) * 256 + lane], u);
     lds_barrier();
 #pragma unroll
@@ -169,7 +211,8 @@ __global__ __launch_bounds__(256) void delta_scan(DeltaDims d, const int32_t* __
           get2(o, next, q, p);
           __builtin_amdgcn_sched_barrier(0);
         }
-        S[q] = BWD ? o.whole * S[q] + o.add[q] - (a0 + a1) : o.whole * S[q] + (a0 + a1);
+        const f32x4 kept = o.whole == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o.whole * S[q];
+        S[q] = BWD ? kept + o.add[q] - (a0 + a1) : kept + (a0 + a1);
       }
     __builtin_amdgcn_sched_barrier(0);
     get_rest(o, next);
@@ -251,11 +294,13 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 4) void delta_out(op
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int s = 16 * is + 4 * g + r;
-        P[is][r] = s <= t ? cfg.scale * decay(gt, t, s) * P[is][r] : 0.f;
+        const float dec = s <= t ? decay(gt, t, s) : 0.f;
+        P[is][r] = dec == 0.f ? 0.f : cfg.scale * dec * P[is][r];
       }
     }
   }
   const float f = cfg.scale * gt.head[t];
+  const int last = gt.last();
 #pragma unroll
   for (int c = 0; c < KT; ++c) qs[c] = row4(&q.v[t][16 * c + 4 * g]) * f;
   __syncthreads();                                     // q and k are done with
@@ -272,7 +317,20 @@ __global__ __launch_bounds__(256, KT * sizeof(T) > 16 ? 2 : 4) void delta_out(op
 #pragma unroll
     for (int is = 0; is < 4; ++is)
       if (is <= w) acc2 = mfma4(P[is], at4(tiles + (KT + is) * 256), acc2);
-    acc += acc2;
+    if (last && __any(!finite(acc + acc2))) {       // tokens 16w + 4g .. + 3: no state behind a reset, and one segment's updates at a time
+      f32x4 sum = only(gt, 0, 16 * w + 4 * g, acc);
+#pragma unroll 1
+      for (int s = gt.first(); s <= last; ++s) {
+        acc2 = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int is = 0; is < 4; ++is)
+          if (is <= w) acc2 = mfma4(P[is], only(gt, s, 16 * is + 4 * g, at4(tiles + (KT + is) * 256)), acc2);
+        sum += only(gt, s, 16 * w + 4 * g, acc2);
+      }
+      acc = sum;
+    } else {
+      acc += acc2;
+    }
     acc = turn4(acc);                      // four columns of one token a lane
     const int tt = 16 * w + 4 * g + (j & 3), v4 = 16 * vt + 4 * (j >> 2);
     if (tt >= a.nv) acc = f32x4{0.f, 0.f, 0.f, 0.f};   // (behind the last live token q is 0, but its product with a state that is not finite is not)

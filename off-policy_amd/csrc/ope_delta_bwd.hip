@@ -50,11 +50,13 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * it + 4 * g + r;
-      acc[r] = t >= s ? cfg.scale * decay(gt, t, s) * acc[r] : 0.f;
+      const float dec = t >= s ? decay(gt, t, s) : 0.f;
+      acc[r] = dec == 0.f ? 0.f : cfg.scale * dec * acc[r];
     }
     put4(&PT[s][16 * it + 4 * g], acc);
   }
   __syncthreads();
+  const int last = gt.last();
   for (int vt = w; vt < d.VT; vt += NW) {
     const int v = 16 * vt + j;
     f32x4 x[4];
@@ -64,15 +66,30 @@ __global__ __launch_bounds__(64 * chunk_waves<KT>(), KT >= 4 ? 4 : 3) void delta
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int it = is; it < 4; ++it) acc = mfma4(at4(&PT[16 * is + j][16 * it + 4 * g]), x[it], acc);
+      if (last && __any(!finite(acc))) {                // one segment at a time
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int s = gt.first(); s <= last; ++s) {
+          f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int it = is; it < 4; ++it) part = mfma4(at4(&PT[16 * is + j][16 * it + 4 * g]), only(gt, s, 16 * it + 4 * g, x[it]), part);
+          acc += only(gt, s, 16 * is + 4 * g, part);
+        }
+      }
       put4(&dUT[((a.c * d.VT + vt) * 4 + is) * 256 + tile_lane()], acc);
     }
 #pragma unroll
-    for (int it = 0; it < 4; ++it) x[it] *= at4(&gt.head[16 * it + 4 * g]) * cfg.scale;
+    for (int it = 0; it < 4; ++it) x[it] = gated(at4(&gt.head[16 * it + 4 * g]) * cfg.scale, x[it]);
 #pragma unroll kPair                                     // (all of an odd number of tiles would be unrolled, into scratch memory)
     for (int kt = 0; kt < KT; ++kt) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int it = 0; it < 4; ++it) acc = mfma4(column4(&q.v[16 * it + 4 * g][16 * kt + j], RS), x[it], acc);
+      if (last && __any(!finite(acc))) {                // nothing of the tokens behind a reset
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int it = 0; it < 4; ++it) acc = mfma4(only(gt, 0, 16 * it + 4 * g, column4(&q.v[16 * it + 4 * g][16 * kt + j], RS)), x[it], acc);
+      }
       put4(&dST[((a.c * d.VT + vt) * KT + kt) * 256 + tile_lane()], acc);
     }
   }
@@ -100,6 +117,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   float(*inv)[16][20] = reinterpret_cast<float(*)[16][20]>(pool + 2 * kC * (kC + 4));
   __shared__ float dbv[2][kC], sums[2][4][kC], dots[8];
   __shared__ Gates gt;
+  __shared__ unsigned long long odd;                   // segments that hold a key or query that is not finite, counted from the first token's
   const ChunkAt a = chunk_at(d, lengths, blockIdx.x);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   const int rows = min(d.T - a.t0, kC), hk = a.h / (d.H / d.Hk);
@@ -144,25 +162,72 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   if (w == 0) load_gates(gt, cfg, a, g_in, beta_in);
   load_rows<T, KT, 512>(q, q_in, cfg.q_stride, a, hk, d.K);
   load_rows<T, KT, 512>(k, k_in, cfg.k_stride, a, hk, d.K);
+  if (threadIdx.x == 0) odd = 0;
   __syncthreads();
   minus_A<T, KT>(NA, k, gt);
+  const int last_seg = gt.last();
+  const int first_seg = gt.first();
+  auto each4 = [&](auto f) {                           // four elements of q and k at (t, f), threads side by side
+    for (int x = threadIdx.x; x < kC * KT * 4; x += 512) f(x / (KT * 4), (x % (KT * 4)) * 4);
+  };
+  if (last_seg)
+    each4([&](int t, int f) {
+      bool fine = true;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = (float)q.v[t][f + e], y = (float)k.v[t][f + e];
+        fine &= x - x == 0.f && y - y == 0.f;
+      }
+      if (!fine) atomicOr(&odd, 1ull << (gt.seg[t] - first_seg));
+    });
   __syncthreads();
-  if (w == 0) diag_inverse(inv, NA);
+  if (w == 0) diag_inverse(inv, NA, gt);
+  if (odd)                                             // A has them; the products over the chunk's tokens below go without (poison)
+    each4([&](int t, int f) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = (float)q.v[t][f + e], y = (float)k.v[t][f + e];
+        if (x - x != 0.f) q.v[t][f + e] = (T)0.f;
+        if (y - y != 0.f) k.v[t][f + e] = (T)0.f;
+      }
+    });
   __syncthreads();
   // dR = (I + A)^-T dU, block backward substitution, 16 value columns a wave at a time; left in dUT with its tiles transposed
-  for (int vt = w; vt < d.VT; vt += 8) {
-    float* at = dUT + (a.c * d.VT + vt) * 4 * 256;
-    f32x4 x[4];
-#pragma unroll
-    for (int it = 0; it < 4; ++it) x[it] = at4(at + it * 256 + tile_lane());
+  auto solve = [&](f32x4* x, auto apart, int seg) {    // as in delta_prep
 #pragma unroll
     for (int it = 3; it >= 0; --it) {
       f32x4 acc = x[it];
 #pragma unroll
       for (int kt = it + 1; kt < 4; ++kt) acc = mfma4(col4(&NA[16 * kt + 4 * g][16 * it + j], kC + 4), x[kt], acc);
+      if (apart()) acc = only(gt, seg, 16 * it + 4 * g, acc);
       x[it] = mfma4(col4(&inv[it][4 * g][j], 20), acc, f32x4{0.f, 0.f, 0.f, 0.f});
-      put4(at + it * 256 + turned_lane(), turn4(x[it]));
+      if (apart()) x[it] = only(gt, seg, 16 * it + 4 * g, x[it]);
     }
+  };
+  for (int vt = w; vt < d.VT; vt += 8) {
+    float* at = dUT + (a.c * d.VT + vt) * 4 * 256;
+    f32x4 x[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it) x[it] = at4(at + it * 256 + tile_lane());
+    solve(x, std::false_type{}, 0);
+    if (last_seg && __any(!finite<4>(x))) {
+      f32x4 b[4], y[4];
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        b[it] = at4(at + it * 256 + tile_lane());
+        x[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll 1
+      for (int s = gt.first(); s <= last_seg; ++s) {
+#pragma unroll
+        for (int it = 0; it < 4; ++it) y[it] = only(gt, s, 16 * it + 4 * g, b[it]);
+        solve(y, std::true_type{}, s);
+#pragma unroll
+        for (int it = 0; it < 4; ++it) x[it] += y[it];
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) put4(at + it * 256 + turned_lane(), turn4(x[it]));
   }
   __syncthreads();     // dR of all columns is in dUT; A is done with
   const int wt = __builtin_amdgcn_readfirstlane(w & 3), half = __builtin_amdgcn_readfirstlane(w >> 2), k0 = half * KH, t = 16 * wt + j;
@@ -255,7 +320,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     for (int r = 0; r < 4; ++r) {
       const int s = 16 * is + 4 * g + r;
       const float dec = s <= t ? decay(gt, t, s) : 0.f;
-      M[is][r] = half ? (s < t ? -M[is][r] * dec : 0.f) : M[is][r] * cfg.scale * dec;
+      M[is][r] = dec == 0.f || (half && s == t) ? 0.f : M[is][r] * (half ? -dec : cfg.scale * dec);
     }
     put4(half ? &dAs[t][16 * is + 4 * g] : &dPs[t][16 * is + 4 * g], M[is]);      // dP scale decay, dA decay (without beta_t)
   }
@@ -263,8 +328,8 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   const float fq = cfg.scale * gt.head[t], fr = gt.head[t], bt = gt.beta[t], tail = gt.tail[t];
 #pragma unroll
   for (int q = 0; q < KH; ++q) {
-    X1[q] *= fq;
-    X2[q] *= -fr;
+    X1[q] = fr == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : X1[q] * fq;
+    X2[q] = fr == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : X2[q] * -fr;
   }
   for (int is = 0; is <= wt; ++is) {
     const f32x4 bp = at4(&dPs[t][16 * is + 4 * g]), ba = at4(&dAs[t][16 * is + 4 * g]);
@@ -276,11 +341,13 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
         X2[q] = mfma4(kc, ba, X2[q]);              // the terms of dk that carry beta_t, without it
       }
   }
+  // A token whose segment holds a key or query that is not finite: NaN, in place of the terms that were left out
+  const float poison = odd >> (gt.seg[t] - first_seg) & 1 ? NAN : 0.f;
   f32x4 C[KH];
 #pragma unroll
-  for (int q = 0; q < KH; ++q) C[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int q = 0; q < KH; ++q) C[q] = f32x4{poison, poison, poison, poison};
   for (int it = wt; it < 4; ++it) {
-    const f32x4 bp = col4(&dPs[16 * it + 4 * g][t], kC + 4), ba = col4(&dAs[16 * it + 4 * g][t], kC + 4) * at4(&gt.beta[16 * it + 4 * g]);
+    const f32x4 bp = col4(&dPs[16 * it + 4 * g][t], kC + 4), ba = gated(col4(&dAs[16 * it + 4 * g][t], kC + 4), at4(&gt.beta[16 * it + 4 * g]));
 #pragma unroll
     for (int i = 0; i < KH; ++i)
       if (k0 + i < KT) {
@@ -293,7 +360,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
   for (int i = 0; i < KH; ++i)
     if (k0 + i < KT) {
       const int f = 16 * (k0 + i) + 4 * g;
-      const f32x4 kv = row4(&k.v[t][f]), qv = row4(&q.v[t][f]), e = X3[i] * tail;
+      const f32x4 kv = row4(&k.v[t][f]), qv = row4(&q.v[t][f]), e = tail == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : X3[i] * tail;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         pq = fmaf(qv[r], X1[i][r], pq);
@@ -301,7 +368,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
         pc = fmaf(kv[r], C[i][r], pc);
         ps = fmaf(kv[r], e[r], ps);
       }
-      put_k(dq, cfg.dq_stride, dqp, t, f, X1[i]);
+      put_k(dq, cfg.dq_stride, dqp, t, f, X1[i] + poison);
       put_k(dk, cfg.dk_stride, dkp, t, f, X2[i] * bt + C[i] + e);
     }
   pq = rowsum4(pq); pr = rowsum4(pr); pc = rowsum4(pc); ps = rowsum4(ps);
@@ -317,7 +384,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     const float r = sums[0][1][l] + sums[1][1][l];
     const float db = r + dbv[0][l] + dbv[1][l];
     if (l < rows) db0[(int64_t)l * cfg.dbeta_stride[1]] = l < a.nv ? db : 0.f;
-    double end = (double)sums[0][3][l] + sums[1][3][l];
+    double end = gt.tail[l] == 0.f ? 0.0 : (double)sums[0][3][l] + sums[1][3][l];
     double x = (double)sums[0][0][l] + sums[1][0][l] + gt.beta[l] * (double)r - sums[0][2][l] - sums[1][2][l] - end;
     for (int m = 1; m < 64; m <<= 1) {
       const double o = __shfl_down(x, m, 64);
@@ -327,7 +394,7 @@ __global__ __launch_bounds__(512, KT * sizeof(T) > 16 ? 2 : 4) void delta_bwd_ma
     }
     double dot_all = 0.0;
     for (int i = 0; i < 8; ++i) dot_all += dots[i];
-    end += (double)gt.whole * dot_all;
+    if (gt.whole != 0.f) end += (double)gt.whole * dot_all;
     if (seg == gt.seg[63]) x += end;
     const bool cut = seg != (l > 0 ? gt.seg[l - 1] : 0);       // g = -inf here
     if (l < rows) dg0[(int64_t)l * cfg.dg_stride[1]] = l < a.nv && !cut ? (float)x : 0.f;

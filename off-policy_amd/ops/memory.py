@@ -119,7 +119,8 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
     q, k [B, T, Hk, K], v [B, T, H, V] of one type (float32, bfloat16, float16), any strides with a contiguous last axis (a time-major batch is
     passed as x.transpose(0, 1)); H is a multiple of Hk and value head h reads query / key head h // (H // Hk). K up to 128, V up to 1024.
     log_decay, beta float32 [B, T, H]: log_decay is at most 0 in use; where exp(log_decay) is 0 in float32 (-inf, the type's lowest value, anything
-    under -103.97) the (finite) state is cleared in front of its token, as where a row of the batch goes on with another episode. initial_state float32 [B, H, K, V] (None: zeros). lengths int32 [B] (None: T): tokens at and behind
+    under -103.97) the state is cleared in front of its token, as where a row of the batch goes on with another episode: nothing of the one reaches the
+    other, not even what is not finite (which inside its own episode may also reach tokens in front of it, within a chunk of 64). initial_state float32 [B, H, K, V] (None: zeros). lengths int32 [B] (None: T): tokens at and behind
     lengths[b] are not read and change nothing, their outputs and gradients are 0. scale: 1 / sqrt(K) where None. Keys have unit length in use:
     the rule needs beta |k|^2 < 2 to stay bounded.
 

@@ -167,6 +167,68 @@ def test_delta_rule_resets_are_exact(ops):
     R.close(first, oa[:, at:at + 58].double(), 0, 2 * delta_terms(32, 32, 140), "second episode alone")
 
 
+@pytest.mark.parametrize("low", [-INF, torch.finfo(F32).min])
+@pytest.mark.parametrize("H,Hk,K,V,dtype", [(2, 1, 24, 20, F32), (2, 2, 128, 40, BF16), (1, 1, 96, 130, F16), (2, 2, 64, 64, F32)])
+def test_what_is_not_finite_stays_in_its_episode(ops, H, Hk, K, V, dtype, low):
+    """A NaN or an infinity in any input or gradient of one episode of a row leaves the other episodes' outputs and gradients what they are, to the bit.
+    Episodes of one chunk, of parts of chunks, of several, and one of three tokens; the initial state is the first's, the final one the last's."""
+    g = gen(56)
+    B, T, starts = 2, 200, [0, 20, 64, 90, 93, 150]
+    ends = starts[1:] + [T]
+    clean = delta_inputs(g, B, T, H, Hk, K, V, dtype)
+    clean[3][:, starts[1:]] = low
+    clean += [randn(g, B, H, K, V), randn(g, B, T, H, V, dtype=dtype), randn(g, B, H, K, V)]
+
+    def run(x):
+        leaves = [t.clone().requires_grad_() for t in x[:6]]
+        o, S = ops.gated_delta_rule(*leaves[:5], initial_state=leaves[5])
+        return (o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [x[6], x[7]]))
+
+    want = run(clean)
+    assert all(t.isfinite().all() for t in want)
+    for e, (a, b) in enumerate(zip(starts, ends)):
+        for i, name in enumerate(("q", "k", "v", "log_decay", "beta", "initial_state", "dout", "dstate")):
+            for value in (math.nan, INF):
+                if name == "initial_state" and e or name == "dstate" and e < len(starts) - 1:
+                    continue
+                x = [t.clone() for t in clean]
+                if name in ("initial_state", "dstate"):
+                    x[i][0, :, K // 2, V // 2] = value
+                else:
+                    x[i][0, (a + b) // 2] = value
+                others = torch.ones(B, T, dtype=torch.bool, device="cuda")
+                others[0, a:b] = False
+                for j, (got, ref) in enumerate(zip(run(x), want)):
+                    if j == 1 or j == 7:             # the final state, the initial state's gradient
+                        same = got, ref
+                        if e == (len(starts) - 1 if j == 1 else 0):
+                            same = got[1], ref[1]
+                    else:
+                        same = got[others], ref[others]
+                    assert torch.equal(*same), (name, e, value, j)
+
+
+def test_a_reset_clears_whatever_the_state_holds(ops):
+    """At the first token of a row, of a chunk, and of a row whose state leaves the range of float32; huge finite keys and queries are no NaN."""
+    g = gen(57)
+    inputs = delta_inputs(g, 2, 140, 2, 2, 32, 32, F32)
+    inputs[3][:, 0] = inputs[3][:, 128] = -INF
+    bad = torch.full((2, 2, 32, 32), math.nan, device="cuda")
+    leaves = [[x.clone().requires_grad_() for x in (*inputs, s)] for s in (bad, torch.zeros_like(bad))]
+    runs = [(*(out := ops.gated_delta_rule(*x[:5], initial_state=x[5])), *torch.autograd.grad(out[0].sum() + out[1].sum(), x)) for x in leaves]
+    for a, b in zip(*runs):
+        assert a.isfinite().all() and torch.equal(a, b)
+    over = [x.clone() for x in inputs]
+    over[4][:, 100:110] = 1e30                       # the state grows past float32 within a few of these
+    o, S = ops.gated_delta_rule(*over)
+    assert not o[:, 100:128].isfinite().all() and torch.equal(o[:, 128:], runs[0][0][:, 128:]) and torch.equal(S, runs[0][1])
+    huge = [x.clone() for x in inputs]
+    huge[0][:, 5], huge[4][:, 5] = 1.2e38, 0.0
+    x = [t.requires_grad_() for t in huge]
+    dk = torch.autograd.grad(ops.gated_delta_rule(*x, scale=1e-38)[0][:, 10:].sum(), x[1])[0]
+    assert dk.isfinite().all()
+
+
 def test_delta_rule_on_repeated_keys_and_full_writes(ops):
     """All keys the same and beta = 1: the triangular system at its worst, every token overwrites the last."""
     g = gen(4)
