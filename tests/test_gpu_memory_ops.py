@@ -601,6 +601,52 @@ def test_linear_relu(ops):
             R.close(a, c, 1, 0, "gradient")
 
 
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,K,N", [(5, 7, 3), (64, 252, 64), (65, 33, 70), (300, 520, 130), (1203, 1101, 1003), (4090, 601, 4090), (4090, 2045, 600), (601, 4090, 4090)])
+def test_linear_loses_nothing_of_whole_numbers(ops, M, K, N, dtype, act):
+    """Products and sums of small whole numbers are exact, so every result is the exact one rounded once: a row, a column or a tail that is left out shows.
+    Few rows, tiles of 64, 128 and 256 with and without splits, in y, dx and dw, all in odd sizes."""
+    g = gen(58)
+    x, w, b, r, dy = (torch.randint(-n, n + 1, s, generator=g, device="cuda").to(dtype) for n, s in ((3, (M, K)), (2, (N, K)), (3, (N,)), (3, (M, N)), (2, (M, N))))
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = ops.linear(x, w, bias=b, residual=r, activation=act)
+    x64, w64, b64, r64, dy64 = (t.detach().double() for t in (x, w, b, r, dy))
+    z = x64 @ w64.t() + b64
+    assert z.abs().max() < 2 ** 20
+    dz = dy64 if act == "none" else torch.where(z > 0, dy64, 0.0)
+    want = ((z if act == "none" else z.clamp_min(0)) + r64, dz @ w64, dz.t() @ x64, dz.sum(0), dy64)
+    for name, got, exact in zip(("y", "dx", "dw", "db", "dr"), (y.detach(), *torch.autograd.grad(y, leaves, dy)), want):
+        assert torch.equal(got, exact.float().to(dtype)), name
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(5, 16, 3), (64, 2048, 96), (65, 130, 70), (300, 1003, 260), (2050, 1040, 2050)])
+def test_linear_on_8_bits_loses_nothing_of_whole_numbers(ops, M, K, N, out):
+    g = gen(59)
+    x, w = (torch.randint(-n, n + 1, s, generator=g, device="cuda").float() for n, s in ((3, (M, K)), (2, (N, K))))
+    xs, ws = (2.0 ** torch.randint(-2, 3, (n,), generator=g, device="cuda").float() for n in (M, N))
+    y = ops.linear_fp8(x.to(E4M3), xs, w.to(E4M3), ws, out_dtype=out)
+    assert torch.equal(y, ((x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()).float().to(out))
+
+
+@pytest.mark.parametrize("M,K,N,dtype,act", [(4090, 600, 2045, BF16, "silu"), (4090, 600, 2045, BF16, "none"), (4090, 520, 4090, F16, "gelu"), (601, 1030, 2050, BF16, "tanh")])
+def test_linear_errors_in_16_bits_are_those_of_their_roundings(ops, M, K, N, dtype, act):
+    """By the norm, where roundings of independent values add up as their squares: one of each dz (none without an activation) and one of each result, each at most
+    half a step u, make at most sqrt(2) u and u of a result whose terms are as independent; 1.6 u and 1.1 u leave room for the sums in float32 and for
+    chance (3 % over some 10^6 values). A single row left out of M = 4090 would be 1.6 % of dw, 4 u in bfloat16."""
+    g = gen(60)
+    x, w, dy = randn(g, M, K, dtype=dtype).requires_grad_(), randn(g, N, K, dtype=dtype, scale=K ** -0.5).requires_grad_(), randn(g, M, N, dtype=dtype)
+    y = ops.linear(x, w, activation=act)
+    x64, w64 = (t.detach().double().requires_grad_() for t in (x, w))
+    y64 = R.linear(x64, w64, act=act)
+    u = R.half_step(dtype)
+    off = lambda a, b: ((a.double() - b).norm() / b.norm()).item()                    # noqa: E731
+    assert off(y.detach(), y64.detach()) <= 1.1 * u
+    for name, a, b in zip(("dx", "dw"), torch.autograd.grad(y, (x, w), dy), torch.autograd.grad(y64, (x64, w64), dy.double())):
+        assert off(a, b) <= (1.1 if act == "none" else 1.6) * u, name
+
+
 def test_linear_wide_tiles(ops):
     """Enough tiles of 128 that the large tile is taken, in whole and in odd sizes."""
     g = gen(33)
