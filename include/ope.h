@@ -758,7 +758,7 @@ int ope_delta_forward(const ope_delta_cfg* cfg, const void* q, const void* k, co
 int ope_delta_backward(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta,
                        const int32_t* lengths, const void* saved, int64_t saved_bytes, const void* d_o, const float* d_state, void* dq,
                        void* dk, void* dv, float* dg, float* dbeta, float* d_state0, void* workspace, int64_t workspace_bytes, void* stream);
-/* One token: cfg->seq_len is not read, the token strides neither; `state` [batch][n_heads][key_dim][value_dim] is updated in place. */
+/* One token: cfg->seq_len is checked as elsewhere (1 will do) and means nothing, the token strides are not read; `state` [batch][n_heads][key_dim][value_dim] is updated in place. */
 int ope_delta_step(const ope_delta_cfg* cfg, const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
                    void* o, void* stream);
 

@@ -1,9 +1,9 @@
 // Shared pieces of the gated delta rule's kernels (ope_delta.hip: forward and one-token step; ope_delta_bwd.hip: gradients).
 //
 // Names: a CHUNK is 64 tokens of one (sequence, head) = "chunk-head" c = (b * H + h) * n + i. Kp / Vp are the key and value widths padded to the
-// tiles of 16 the kernels work in (Kp: 16 to 96, or 128). Arithmetic is float32 throughout, on the f32 matrix instruction of ope_common.h:
-// its "transposed chain" (lane (j, g) holds features 4g .. 4g+3 of data row j) is both the form a product leaves and the form the next one
-// reads, so the triangular solve and the scan need no shuffles.
+// tiles of 16 the kernels work in (Kp: 16 to 96, or 128). Every sum is float32. What touches a state, a decay or a solve runs on the f32 matrix
+// instruction of ope_common.h: its "transposed chain" (lane (j, g) holds features 4g .. 4g+3 of data row j) is both the form a product leaves and the
+// form the next one reads, so the triangular solve and the scan need no shuffles. q k^T and k k^T of 16-bit inputs run on the bf16 / f16 one (dot4).
 //
 // Arrays in `saved` (S, kept for the backward pass) and in the workspace (W). All lie in TILES of 16 x 16, in the order in which the lanes of a
 // wave hold them: lane (j, g) has row j, columns 4g .. 4g+3, tile after tile, so that every access of a wave is one run of whole cache lines (rows

@@ -1,7 +1,7 @@
 // Linear layer with bias, activation and residual in its epilogue, and its gradients (ope_linear, ope_linear_backward; ope.h).
 //
-// One product kernel for all four operand types: C[m][n] = sum_k A[m][k] B[n][k], both operands with the contraction running along memory.
-// It counts in BYTES of k: a lane takes 16 bytes of one row -- 4 float32, 8 bfloat16 / float16 or 16 e4m3 values -- and feeds them to the matrix
+// One product kernel for all four operand types: C[m][n] = sum_k A[m][k] B[n][k]. In the forward product the contraction runs along memory in both operands;
+// in the gradients' (dz w, dz^T x) over the rows of one or both, which are turned in registers (Loader). It counts in BYTES of k: a lane takes 16 bytes of one row -- 4 float32, 8 bfloat16 / float16 or 16 e4m3 values -- and feeds them to the matrix
 // instructions of that type (the same permutation of k on both operands, so any grouping is right). The weight row is the instruction's A
 // operand: a lane then holds 4 consecutive columns of one output row, and the epilogue reads and writes packs.
 #include <type_traits>

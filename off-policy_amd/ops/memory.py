@@ -125,8 +125,8 @@ def gated_delta_rule(q, k, v, log_decay, beta, initial_state=None, lengths=None,
     the rule needs beta |k|^2 < 2 to stay bounded.
 
     Returns (out [B, T, H, V] of q's type, final state float32 [B, H, K, V]); differentiable in q, k, v, log_decay (0 where it clears), beta and
-    initial_state, once (no create_graph). The backward pass keeps per 64 tokens and head one state and the tokens' updates in float32:
-    (K V + 64 (K + V)) * 4 bytes."""
+    initial_state, once (no create_graph). Beside its inputs, the backward pass keeps per 64 tokens (or part of them) and head one state, the tokens' updates and
+    their decays in float32: (Kp Vp + 64 (Kp + Vp) + 65) * 4 bytes, with Kp and Vp the widths rounded up to 16 (Kp: to 128 above 96)."""
     plain_call(q, k, v, log_decay, beta, initial_state)
     plan = _check(q, k, v, log_decay, beta, initial_state, lengths, 2)
     scale = float(plan[4] ** -0.5 if scale is None else scale)
