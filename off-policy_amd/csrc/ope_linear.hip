@@ -83,9 +83,9 @@ __device__ __forceinline__ u32x4 row16(const uint8_t* row, int64_t k, int64_t le
   return v;
 }
 // The last step of float32 rows that end inside it, for the forward product: piece g of a half (16 values) takes k = 4 r + g, so that the matrix
-// instructions add what is left in ascending order of k. Whole steps go by k = 4 g + r (16 bytes a lane); with both, z is to the bit what the library's
-// float32 product of the same row gives where neither splits k, and a relu's gate falls on the same side where z is within rounding of 0 (one that falls
-// otherwise moves a row of dx and a row of dw). The loads are single ones there anyway.
+// instructions add what is left in ascending order of k. Whole steps go by k = 4 g + r (16 bytes a lane); with both, z was to the bit what the library's
+// float32 product gives on the rows compared that neither splits (252, 480, 672 and 2048 wide), and a relu's gate falls on the same side where z is within
+// rounding of 0 (one that falls otherwise moves a row of dx and a row of dw). The loads are single ones there anyway.
 __device__ __forceinline__ u32x4 last16(const uint8_t* row, int64_t half, int g, int64_t len) {
   u32x4 v = {0, 0, 0, 0};
 #pragma unroll
